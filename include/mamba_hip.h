@@ -715,6 +715,114 @@ typedef struct MambaCast {
 } MambaCast;
 int mamba_cast_bf16(const MambaCast *c, int count, mamba_stream_t stream);
 
+/* -------------------------------------------------------------------------
+ * Gated linear recurrence, one state per channel, over rows of a batch or over packed sequences:
+ *   r = sigmoid(gate_a), i = sigmoid(gate_x), k = rate * softplus(decay[channel]), log a = -k r
+ *   h_t = a_t h_{t-1} + sqrt(1 - a_t^2) i_t x_t,   out_t = h_t
+ * x, gate_a, gate_x, out and their gradients are (batch, seqlen, dim) of `dtype`, unit channel stride, batch and
+ * position strides given (any alignment).  decay (dim) is of decay_dtype.  States are dense fp32: (batch, dim), or
+ * (nseq, dim) with cu_seqlens.
+ * cu_seqlens (nseq + 1 int32, batch 1) packs nseq sequences into the row: sequence q has the positions
+ * cu_seqlens[q] .. cu_seqlens[q + 1] - 1 (none where the two are equal) and starts from its own initial state.
+ * Positions before the first and behind the last sequence are read but count for nothing, whatever they hold: their
+ * outputs and gradients are 0.  The values are compared, never used as addresses.
+ * The forward call leaves in `ckpt` what the backward call of the same tensors needs; gated_scan_ckpt_bytes and
+ * gated_scan_bwd_ws_bytes give the bytes of ckpt and of the backward workspace `ws`, both 16-byte aligned, contents
+ * ignored on entry.  Nothing is kept between calls and every result repeats bit for bit.
+ * ------------------------------------------------------------------------- */
+typedef struct GatedScanParams {
+  int32_t batch, seqlen, dim;
+  int32_t nseq; /* 0: the rows of the batch are the sequences */
+  int32_t dtype, decay_dtype;
+  float rate;
+  int32_t reserved;
+  const void *x, *gate_a, *gate_x;
+  const void *decay;
+  const float *initial_states; /* nullable: zeros */
+  const int32_t *cu_seqlens;   /* null iff nseq is 0 */
+  void *out;                   /* forward only */
+  float *final_states;         /* forward only, nullable */
+  void *ckpt;
+  int64_t x_bs, x_ls, gate_a_bs, gate_a_ls, gate_x_bs, gate_x_ls, out_bs, out_ls;
+  /* ---- backward only ---- */
+  const void *dout;
+  const float *dfinal_states; /* nullable */
+  void *dx, *dgate_a, *dgate_x;
+  void *ddecay;           /* of decay_dtype */
+  float *dinitial_states; /* nullable */
+  void *ws;
+  int64_t dout_bs, dout_ls, dx_bs, dx_ls, dgate_a_bs, dgate_a_ls, dgate_x_bs, dgate_x_ls;
+} GatedScanParams;
+
+int64_t gated_scan_ckpt_bytes(const GatedScanParams *p);
+int64_t gated_scan_bwd_ws_bytes(const GatedScanParams *p);
+int gated_scan_fwd(const GatedScanParams *p, mamba_stream_t stream);
+int gated_scan_bwd(const GatedScanParams *p, mamba_stream_t stream);
+
+/* One position of the same recurrence: state (state_rows, dim) is updated in place, out (batch, dim) is the new state
+ * in dtype.  Row state_batch_indices[b] of the state belongs to entry b (row b without them); an index outside
+ * [0, state_rows) is a padding entry: no state is touched, out is 0.  The rows named have to be different ones.
+ * Unit channel strides. */
+typedef struct GatedStepParams {
+  int32_t batch, dim, state_rows;
+  int32_t dtype, state_dtype, decay_dtype;
+  float rate;
+  int32_t reserved;
+  void *state;
+  const void *x, *gate_a, *gate_x;
+  const void *decay;
+  const int32_t *state_batch_indices; /* nullable */
+  void *out;
+  int64_t state_rs, x_rs, gate_a_rs, gate_x_rs, out_rs;
+} GatedStepParams;
+
+int gated_state_update(const GatedStepParams *p, mamba_stream_t stream);
+
+/* -------------------------------------------------------------------------
+ * The norm behind a block, its gate and residual scale, the residual add and the norm in front of the next block, in
+ * one pass over the rows:
+ *   s = residual + scale * norm(x; norm_weight, norm_bias) * silu(z);   residual_out = s
+ *   out = norm(s; next_weight, next_bias)
+ * norm is LayerNorm or RMSNorm (is_rms) over the row, out the norm of s before s is rounded to res_dtype.
+ * x, z, out, dout, dx, dz are (rows, dim) of `dtype`; residual, residual_out, dsum (the gradient of residual_out),
+ * dresidual of res_dtype (dtype or fp32); unit channel stride, row strides given.  The parameters (dim) and their
+ * gradients are of weight_dtype; without `scale` the factor is scale_value.
+ * stats: fp32 (rows, 4), written by the forward call (nullable there) and read by the backward call, which forms s
+ * again from x, z and residual.  parts: fp32 workspace of nparts * nsums * dim, nsums = 2, + 1 with scale, + 1 for
+ * each bias; nparts in 1..65536 (norm_block_bwd_nparts gives the number that suits).  dim <= 32768.
+ * ------------------------------------------------------------------------- */
+typedef struct NormBlockParams {
+  int32_t rows, dim;
+  int32_t dtype, res_dtype, weight_dtype;
+  int32_t is_rms;
+  int32_t nparts; /* backward only */
+  float eps;
+  float scale_value;
+  int32_t reserved;
+  const void *x;
+  const void *z; /* nullable: no gate */
+  const void *residual;
+  const void *norm_weight, *next_weight;
+  const void *norm_bias, *next_bias; /* nullable */
+  const void *scale;                 /* nullable */
+  void *out, *residual_out;          /* forward only */
+  float *stats;
+  int64_t x_rs, z_rs, residual_rs, out_rs, residual_out_rs;
+  /* ---- backward only ---- */
+  const void *dout;
+  const void *dsum; /* nullable */
+  void *dx, *dresidual;
+  void *dz; /* null iff z is null */
+  void *dnorm_weight, *dnext_weight;
+  void *dnorm_bias, *dnext_bias, *dscale; /* null iff the parameter is null */
+  float *parts;
+  int64_t dout_rs, dsum_rs, dx_rs, dz_rs, dresidual_rs;
+} NormBlockParams;
+
+int norm_block_fwd(const NormBlockParams *p, mamba_stream_t stream);
+int norm_block_bwd(const NormBlockParams *p, mamba_stream_t stream);
+int norm_block_bwd_nparts(const NormBlockParams *p);
+
 #ifdef __cplusplus
 }
 #endif

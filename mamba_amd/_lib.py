@@ -137,6 +137,40 @@ class NormResidualParams(ctypes.Structure):
     )
 
 
+class GatedScanParams(ctypes.Structure):
+    _fields_ = (
+        [(n, c_i32) for n in ("batch", "seqlen", "dim", "nseq", "dtype", "decay_dtype")]
+        + [("rate", c_f32), ("reserved", c_i32)]
+        + [(n, c_vp) for n in ("x", "gate_a", "gate_x", "decay", "initial_states", "cu_seqlens", "out", "final_states", "ckpt")]
+        + [(n, c_i64) for n in ("x_bs", "x_ls", "gate_a_bs", "gate_a_ls", "gate_x_bs", "gate_x_ls", "out_bs", "out_ls")]
+        + [(n, c_vp) for n in ("dout", "dfinal_states", "dx", "dgate_a", "dgate_x", "ddecay", "dinitial_states", "ws")]
+        + [(n, c_i64) for n in ("dout_bs", "dout_ls", "dx_bs", "dx_ls", "dgate_a_bs", "dgate_a_ls", "dgate_x_bs",
+                                "dgate_x_ls")]
+    )
+
+
+class GatedStepParams(ctypes.Structure):
+    _fields_ = (
+        [(n, c_i32) for n in ("batch", "dim", "state_rows", "dtype", "state_dtype", "decay_dtype")]
+        + [("rate", c_f32), ("reserved", c_i32)]
+        + [(n, c_vp) for n in ("state", "x", "gate_a", "gate_x", "decay", "state_batch_indices", "out")]
+        + [(n, c_i64) for n in ("state_rs", "x_rs", "gate_a_rs", "gate_x_rs", "out_rs")]
+    )
+
+
+class NormBlockParams(ctypes.Structure):
+    _fields_ = (
+        [(n, c_i32) for n in ("rows", "dim", "dtype", "res_dtype", "weight_dtype", "is_rms", "nparts")]
+        + [("eps", c_f32), ("scale_value", c_f32), ("reserved", c_i32)]
+        + [(n, c_vp) for n in ("x", "z", "residual", "norm_weight", "next_weight", "norm_bias", "next_bias", "scale", "out",
+                               "residual_out", "stats")]
+        + [(n, c_i64) for n in ("x_rs", "z_rs", "residual_rs", "out_rs", "residual_out_rs")]
+        + [(n, c_vp) for n in ("dout", "dsum", "dx", "dresidual", "dz", "dnorm_weight", "dnext_weight", "dnorm_bias",
+                               "dnext_bias", "dscale", "parts")]
+        + [(n, c_i64) for n in ("dout_rs", "dsum_rs", "dx_rs", "dz_rs", "dresidual_rs")]
+    )
+
+
 _lib = None
 
 
@@ -223,6 +257,18 @@ def load():
     lib.mamba_hip_rows_probe.argtypes = [ctypes.POINTER(c_vp), ctypes.c_int, ctypes.POINTER(c_vp), ctypes.c_int,
                                          ctypes.c_int, ctypes.c_int, c_vp]
     lib.mamba_hip_rows_probe.restype = ctypes.c_int64
+    for name, params in (("gated_scan_fwd", GatedScanParams), ("gated_scan_bwd", GatedScanParams),
+                         ("gated_state_update", GatedStepParams), ("norm_block_fwd", NormBlockParams),
+                         ("norm_block_bwd", NormBlockParams)):
+        fn = getattr(lib, name)
+        fn.argtypes = [ctypes.POINTER(params), c_vp]
+        fn.restype = ctypes.c_int
+    lib.norm_block_bwd_nparts.argtypes = [ctypes.POINTER(NormBlockParams)]
+    lib.norm_block_bwd_nparts.restype = ctypes.c_int
+    for name in ("gated_scan_ckpt_bytes", "gated_scan_bwd_ws_bytes"):
+        fn = getattr(lib, name)
+        fn.argtypes = [ctypes.POINTER(GatedScanParams)]
+        fn.restype = c_i64
     for name in ("norm_residual_fwd", "norm_residual_bwd"):
         fn = getattr(lib, name)
         fn.argtypes = [ctypes.POINTER(NormResidualParams), c_vp]
