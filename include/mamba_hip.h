@@ -788,8 +788,8 @@ int gated_state_update(const GatedStepParams *p, mamba_stream_t stream);
  * dresidual of res_dtype (dtype or fp32); unit channel stride, row strides given.  The parameters (dim) and their
  * gradients are of weight_dtype; without `scale` the factor is scale_value.
  * stats: fp32 (rows, 4), written by the forward call (nullable there) and read by the backward call, which forms s
- * again from x, z and residual.  parts: fp32 workspace of nparts * nsums * dim, nsums = 2, + 1 with scale, + 1 for
- * each bias; nparts in 1..65536 (norm_block_bwd_nparts gives the number that suits).  dim <= 32768.
+ * again from x, z and residual.  parts: fp32 workspace of nparts * nsums * dim, nsums = 2, + 1 for each bias; nparts in
+ * 1..65536 (norm_block_bwd_nparts gives the number that suits).  dim <= 32768.
  * ------------------------------------------------------------------------- */
 typedef struct NormBlockParams {
   int32_t rows, dim;

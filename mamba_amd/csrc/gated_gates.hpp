@@ -14,40 +14,24 @@ template <typename P> DEVI float decay_slope(const P &p, int c) {  // dk / ddeca
   return p.rate / (1.f + expf(-ld_param(p.decay, p.decay_dtype, c)));
 }
 
-// 1 - exp(-v) for v >= 0 without cancellation: the series up to v^7 (next term below 2e-7 of the sum at v = 0.5),
-// beyond it the difference, with ev = exp(-v).
-DEVI float one_minus_exp(float v, float ev) {
-  float s = __builtin_fmaf(v, 1.f / 5040.f, -1.f / 720.f);
-  s = __builtin_fmaf(v, s, 1.f / 120.f);
-  s = __builtin_fmaf(v, s, -1.f / 24.f);
-  s = __builtin_fmaf(v, s, 1.f / 6.f);
-  s = __builtin_fmaf(v, s, -0.5f);
-  s = __builtin_fmaf(v, s, 1.f) * v;
-  return v < 0.5f ? s : 1.f - ev;
-}
-
-// One position: six instructions at quarter rate (two exponentials and two reciprocals of the sigmoids, the exponential
-// of the decay, one reciprocal square root) and ~20 others.
+// One position's gates from kr's factor k and k2 = -k log2(e): r, i, a and m^2 = 1 - a^2.
+//   1 - exp(-2 w) = 2 exp(-w) sinh(w), w = k r: no cancellation where a is near 1, and its series needs two terms below
+// w = 0.25 (the next one is 5e-8 of the sum); from there on 1 - a^2 as it stands.
+// Five of a position's six quarter-rate instructions (two exponentials and two reciprocals for the sigmoids, the
+// exponential of the decay), with the root of m^2 the sixth.
 struct Gates {
-  float r, i, a, m, im;  // im = 1 / m, 0 where m is 0
-  DEVI Gates(float ga, float gx, float k) {
+  float r, i, a, m2;
+  DEVI Gates(float ga, float gx, float k, float k2) {
     r = sigmoid_f(ga);
     i = sigmoid_f(gx);
-    const float kr = k * r;
-    a = fast_exp(-kr);
-    const float m2 = one_minus_exp(2.f * kr, a * a);
-    im = m2 > 0.f ? __builtin_amdgcn_rsqf(m2) : 0.f * m2;  // (a NaN stays one)
-    m = m2 * im;
+    const float w = k * r, w2 = w * w;
+    a = __builtin_amdgcn_exp2f(k2 * r);
+    const float s = __builtin_fmaf(w2, __builtin_fmaf(w2, 1.f / 60.f, 1.f / 3.f), 2.f);
+    m2 = w < 0.25f ? a * w * s : __builtin_fmaf(-a, a, 1.f);
   }
-  // Gradients of one position from g, the gradient of h, and h of the position before.  Where m is 0 (a gate shut to
-  // the last bit, a decay of 0) r / m tends to 0 like sqrt(r), which im = 0 gives.
-  DEVI void grads(float g, float hprev, float x, float k, float &dx, float &dga, float &dgx, float &e) const {
-    const float gm = g * m;
-    dx = gm * i;
-    dgx = dx * x * (1.f - i);
-    e = g * a * (a * i * x * (r * im) - hprev * r);
-    dga = k * (1.f - r) * e;
-  }
+  DEVI float m() const { return __builtin_amdgcn_sqrtf(m2); }
+  // 1 / m, 0 where m is 0 (a gate shut to the last bit, a decay of 0): r / m tends to 0 there like sqrt(r)
+  DEVI float im() const { return m2 > 0.f ? __builtin_amdgcn_rsqf(m2) : 0.f * m2; }  // (a NaN stays one)
 };
 
 }  // namespace

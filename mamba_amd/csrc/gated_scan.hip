@@ -13,23 +13,35 @@
 
 namespace {
 
-template <typename T, bool EVEN, bool PACKED, int R, int NW>
+// The decay's constants of a lane's channels.
+template <int V> struct Rates {
+  Vec<V> d, k, k2;
+  DEVI Rates(const GatedScanParams &p, int c) {
+#pragma unroll
+    for (int e = 0; e < V; ++e) d[e] = ld_param(p.decay, p.decay_dtype, min(c + e, p.dim - 1));
+  }
+  DEVI void form(float rate) {  // once the rows have been asked for
+#pragma unroll
+    for (int e = 0; e < V; ++e) k[e] = rate * softplus_exact(d[e]), k2[e] = -k[e] * kLog2e;
+  }
+};
+
+template <typename T, int V, bool WHOLE, bool PACKED, int R, int NW>
 __global__ __launch_bounds__(NW * 64) void gated_fwd_kernel(const GatedScanParams p, const Chain q, float *ckpt, int ck_rows, int ck_tiles) {
-  __shared__ f32x4 steps[NW][64];
-  __shared__ f32x2 enter[64];
+  __shared__ WaveSteps<V, NW> steps;
+  __shared__ Vec<V> enter[64];
   __shared__ int ticket;
-  const int cgroups = (p.dim + kTileChannels - 1) / kTileChannels, nchains = cgroups * p.batch;
+  const int cgroups = (p.dim + 64 * V - 1) / (64 * V), nchains = cgroups * p.batch;
   const int chain = blockIdx.x % nchains, b = chain / cgroups;
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), cl = lane * 2;
-  const int c = (chain % cgroups) * kTileChannels + cl, L = p.seqlen;
-  const Lane<T, EVEN> at(c, p.dim);
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), L = p.seqlen;
+  const Lane<T, V, WHOLE> at((chain % cgroups) * (64 * V) + lane * V, p.dim);
   const int n = take_tile(q, chain, &ticket);
   const int t0 = (n * NW + wave) * R, rows = min(max(L - t0, 0), R);
-  const float d0 = ld_param(p.decay, p.decay_dtype, min(c, p.dim - 1)), d1 = ld_param(p.decay, p.decay_dtype, min(c + 1, p.dim - 1));
+  Rates<V> rate(p, at.c);
   const T *xp = static_cast<const T *>(p.x) + b * p.x_bs;
   const T *ap = static_cast<const T *>(p.gate_a) + b * p.gate_a_bs;
   const T *gp = static_cast<const T *>(p.gate_x) + b * p.gate_x_bs;
-  Pair<T> x[R], ga[R], gx[R];
+  Raw<T, V> x[R], ga[R], gx[R];
 #pragma unroll
   for (int j = 0; j < R; ++j) {
     const int64_t t = min(t0 + j, L - 1);
@@ -38,85 +50,87 @@ __global__ __launch_bounds__(NW * 64) void gated_fwd_kernel(const GatedScanParam
     x[j] = at.load(xp + t * p.x_ls);
   }
   SeqRows<PACKED ? R : 1> rowsof(PACKED ? p.cu_seqlens : nullptr, PACKED ? p.nseq : -1, t0, L);
-  const float k0 = p.rate * softplus_exact(d0), k1 = p.rate * softplus_exact(d1);
-  f32x2 a[R], bt[R];
-  Step own = no_step();
+  rate.form(p.rate);
+  Step<V> pos[R], own = no_step<V>();
 #pragma unroll
   for (int j = 0; j < R; ++j) {
-    const Gates q0(ga[j].lo(), gx[j].lo(), k0), q1(ga[j].hi(), gx[j].hi(), k1);
-    a[j] = PACKED ? f32x2{fmaxf(q0.a, kTiny), fmaxf(q1.a, kTiny)} : f32x2{q0.a, q1.a};
-    bt[j] = f32x2{q0.m * q0.i * x[j].lo(), q1.m * q1.i * x[j].hi()};
+#pragma unroll
+    for (int e = 0; e < V; ++e) {
+      const Gates g(ga[j].get(e), gx[j].get(e), rate.k[e], rate.k2[e]);
+      pos[j].a[e] = PACKED ? fmaxf(g.a, kTiny) : g.a;
+      pos[j].b[e] = g.m() * g.i * x[j].get(e);
+    }
     if constexpr (PACKED) {
       if (!(rowsof.in >> j & 1)) {
-        a[j] = bt[j] = f32x2{0.f, 0.f};
+        pos[j].a = pos[j].b = vec_of<V>(0.f);
       } else if (rowsof.start >> j & 1) {
-        if (p.initial_states) {
-          const f32x2 h = at.load_state(p.initial_states + (int64_t)rowsof.seq[j] * p.dim, c);
-          bt[j] = f32x2{__builtin_fmaf(a[j].x, h.x, bt[j].x), __builtin_fmaf(a[j].y, h.y, bt[j].y)};
-        }
-        a[j] = f32x2{0.f, 0.f};
+        if (p.initial_states) pos[j].b = apply<false>(pos[j], at.load_state(p.initial_states + (int64_t)rowsof.seq[j] * p.dim));
+        pos[j].a = vec_of<V>(0.f);
       }
     } else {
-      if (j >= rows) a[j] = f32x2{1.f, 1.f}, bt[j] = f32x2{0.f, 0.f};
+      if (j >= rows) pos[j] = no_step<V>();
     }
-    own = then<PACKED>(own, Step{a[j], bt[j]});
+    own = then<PACKED>(own, pos[j]);
   }
-  steps[wave][lane] = f32x4{own.a.x, own.a.y, own.b.x, own.b.y};
+  steps.put(wave, lane, own);
   lds_barrier();
-  Step before = no_step();
-  for (int w = 0; w < wave; ++w) {
-    const f32x4 s = steps[w][lane];
-    before = then<PACKED>(before, Step{f32x2{s.x, s.y}, f32x2{s.z, s.w}});
-  }
-  if (wave == NW - 1) leave_step(q, chain, n, cl, then<PACKED>(before, own));
+  Step<V> before = no_step<V>();
+  for (int w = 0; w < wave; ++w) before = then<PACKED>(before, steps.get(w, lane));
+  if (wave == NW - 1) leave_step(q, chain, n, lane, then<PACKED>(before, own));
   if (wave == 0) {
-    f32x2 first = {0.f, 0.f};
-    if (!PACKED && p.initial_states) first = at.load_state(p.initial_states + (int64_t)b * p.dim, c);
-    enter[lane] = entering<PACKED>(q, chain, n, cl, first);
+    Vec<V> first = vec_of<V>(0.f);
+    if (!PACKED && p.initial_states) first = at.load_state(p.initial_states + (int64_t)b * p.dim);
+    enter[lane] = entering<PACKED>(q, chain, n, lane, first);
   }
   lds_barrier();
-  f32x2 h = apply<PACKED>(before, enter[lane]);
-  if (wave == NW - 1) leave_state(q, chain, n, cl, apply<PACKED>(own, h));
-  if (t0 % ck_rows == 0 && rows > 0) *reinterpret_cast<f32x2 *>(ckpt + ((int64_t)chain * ck_tiles + t0 / ck_rows) * kTileChannels + cl) = h;
+  Vec<V> h = apply<PACKED>(before, enter[lane]);
+  if (wave == NW - 1) leave_state(q, chain, n, lane, apply<PACKED>(own, h));
+  if (t0 % ck_rows == 0 && rows > 0) {
+    float *ck = ckpt + (((int64_t)chain * ck_tiles + t0 / ck_rows) * 64 + lane) * V;
+#pragma unroll
+    for (int e = 0; e < V; ++e) ck[e] = h[e];
+  }
   T *op = static_cast<T *>(p.out) + b * p.out_bs;
 #pragma unroll
   for (int j = 0; j < R; ++j) {
-    h = apply<PACKED>(Step{a[j], bt[j]}, h);
-    if (j < rows) at.store(op + (int64_t)(t0 + j) * p.out_ls, c, h.x, h.y);
+    h = apply<PACKED>(pos[j], h);
+    if (j < rows) at.store(op + (int64_t)(t0 + j) * p.out_ls, h);
     if constexpr (PACKED) {
-      if (p.final_states && (rowsof.last >> j & 1)) at.store_state(p.final_states + (int64_t)rowsof.seq[j] * p.dim, c, h);
+      if (p.final_states && (rowsof.last >> j & 1)) at.store_state(p.final_states + (int64_t)rowsof.seq[j] * p.dim, h);
     }
   }
-  if (!PACKED && p.final_states && t0 < L && t0 + R >= L) at.store_state(p.final_states + (int64_t)b * p.dim, c, h);
+  if (!PACKED && p.final_states && t0 < L && t0 + R >= L) at.store_state(p.final_states + (int64_t)b * p.dim, h);
   if constexpr (PACKED) {
     if (p.final_states && n == 0)
       empty_sequences(p.cu_seqlens, p.nseq, L, [&](int s) {
         const int64_t o = (int64_t)s * p.dim;
-        at.store_state(p.final_states + o, c, p.initial_states ? at.load_state(p.initial_states + o, c) : f32x2{0.f, 0.f});
+        at.store_state(p.final_states + o, p.initial_states ? at.load_state(p.initial_states + o) : vec_of<V>(0.f));
       });
   }
 }
 
 // Tiles from the last one on: what enters a tile is a_t g_t of the position behind it.
-template <typename T, bool EVEN, bool PACKED, int R, int NW>
+template <typename T, int V, bool WHOLE, bool PACKED, int R, int NW>
 __global__ __launch_bounds__(NW * 64) void gated_bwd_kernel(const GatedScanParams p, const Chain q, const float *ckpt, float *parts) {
-  __shared__ f32x4 steps[NW][64], back[NW][64];
-  __shared__ f32x2 enter[64];
+  __shared__ WaveSteps<V, NW> steps, back;
+  __shared__ Vec<V> enter[64];
   __shared__ int ticket;
-  const int cgroups = (p.dim + kTileChannels - 1) / kTileChannels, nchains = cgroups * p.batch;
+  const int cgroups = (p.dim + 64 * V - 1) / (64 * V), nchains = cgroups * p.batch;
   const int chain = blockIdx.x % nchains, b = chain / cgroups;
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), cl = lane * 2;
-  const int c = (chain % cgroups) * kTileChannels + cl, L = p.seqlen;
-  const Lane<T, EVEN> at(c, p.dim);
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), L = p.seqlen;
+  const Lane<T, V, WHOLE> at((chain % cgroups) * (64 * V) + lane * V, p.dim);
   const int n = take_tile(q, chain, &ticket), tile = q.ntiles - 1 - n;
   const int t0 = (tile * NW + wave) * R, rows = min(max(L - t0, 0), R);
-  const float d0 = ld_param(p.decay, p.decay_dtype, min(c, p.dim - 1)), d1 = ld_param(p.decay, p.decay_dtype, min(c + 1, p.dim - 1));
-  const f32x2 saved = *reinterpret_cast<const f32x2 *>(ckpt + ((int64_t)chain * q.ntiles + tile) * kTileChannels + cl);
+  Rates<V> rate(p, at.c);
+  Vec<V> h;
+  const float *ck = ckpt + (((int64_t)chain * q.ntiles + tile) * 64 + lane) * V;
+#pragma unroll
+  for (int e = 0; e < V; ++e) h[e] = ck[e];
   const T *xp = static_cast<const T *>(p.x) + b * p.x_bs;
   const T *ap = static_cast<const T *>(p.gate_a) + b * p.gate_a_bs;
   const T *gp = static_cast<const T *>(p.gate_x) + b * p.gate_x_bs;
   const T *dp = static_cast<const T *>(p.dout) + b * p.dout_bs;
-  Pair<T> x[R], ga[R], gx[R], dout[R];
+  Raw<T, V> x[R], ga[R], gx[R], dout[R];
 #pragma unroll
   for (int j = 0; j < R; ++j) {
     const int64_t t = min(t0 + j, L - 1);
@@ -129,118 +143,130 @@ __global__ __launch_bounds__(NW * 64) void gated_bwd_kernel(const GatedScanParam
   auto starts = [&](int j) { return PACKED && (rowsof.start >> j & 1); };
   auto ends = [&](int j) { return PACKED && (rowsof.last >> j & 1); };
   auto counts = [&](int j) { return PACKED ? (rowsof.in >> j & 1) != 0 : j < rows; };
-  auto initial = [&](int j) {
-    return p.initial_states ? at.load_state(p.initial_states + (int64_t)rowsof.seq[PACKED ? j : 0] * p.dim, c) : f32x2{0.f, 0.f};
-  };
-  const float k0 = p.rate * softplus_exact(d0), k1 = p.rate * softplus_exact(d1);
-  // per position: a, r, m i, x, i and, first r / m, then e / g
-  f32x2 a[R], r[R], i[R], m[R], f[R], xs[R], d[R];
-  Step own = no_step();
+  auto state_of = [&](int j) { return (int64_t)rowsof.seq[PACKED ? j : 0] * p.dim; };
+  auto initial = [&](int j) { return p.initial_states ? at.load_state(p.initial_states + state_of(j)) : vec_of<V>(0.f); };
+  rate.form(p.rate);
+  // of every position: a, r, i, m, x, the gradient that arrives there, and f: first r / m, then e / g
+  Vec<V> a[R], r[R], i[R], m[R], f[R], xs[R], d[R];
+  Step<V> own = no_step<V>();
 #pragma unroll
   for (int j = 0; j < R; ++j) {
-    const Gates q0(ga[j].lo(), gx[j].lo(), k0), q1(ga[j].hi(), gx[j].hi(), k1);
-    a[j] = PACKED ? f32x2{fmaxf(q0.a, kTiny), fmaxf(q1.a, kTiny)} : f32x2{q0.a, q1.a}, r[j] = f32x2{q0.r, q1.r}, i[j] = f32x2{q0.i, q1.i}, m[j] = f32x2{q0.m, q1.m};
-    f[j] = f32x2{q0.r * q0.im, q1.r * q1.im};
-    xs[j] = f32x2{x[j].lo(), x[j].hi()}, d[j] = f32x2{dout[j].lo(), dout[j].hi()};
+#pragma unroll
+    for (int e = 0; e < V; ++e) {
+      const Gates g(ga[j].get(e), gx[j].get(e), rate.k[e], rate.k2[e]);
+      const float im = g.im();
+      a[j][e] = PACKED ? fmaxf(g.a, kTiny) : g.a;
+      r[j][e] = g.r, i[j][e] = g.i, m[j][e] = g.m2 * im, f[j][e] = g.r * im;
+      xs[j][e] = x[j].get(e), d[j][e] = dout[j].get(e);
+    }
     if (!counts(j)) {
       // a position past the row hands everything on, one outside of the sequences nothing
-      a[j] = PACKED ? f32x2{0.f, 0.f} : f32x2{1.f, 1.f};
-      r[j] = m[j] = i[j] = f[j] = xs[j] = d[j] = f32x2{0.f, 0.f};
+      a[j] = vec_of<V>(PACKED ? 0.f : 1.f);
+      r[j] = m[j] = i[j] = f[j] = xs[j] = d[j] = vec_of<V>(0.f);
     }
     if (ends(j) && p.dfinal_states) {
-      const f32x2 v = at.load_state(p.dfinal_states + (int64_t)rowsof.seq[PACKED ? j : 0] * p.dim, c);
-      d[j] = f32x2{d[j].x + v.x, d[j].y + v.y};
+      const Vec<V> v = at.load_state(p.dfinal_states + state_of(j));
+#pragma unroll
+      for (int e = 0; e < V; ++e) d[j][e] += v[e];
     }
-    Step s = {a[j], f32x2{m[j].x * i[j].x * xs[j].x, m[j].y * i[j].y * xs[j].y}};
+    Step<V> s;
+    s.a = a[j];
+#pragma unroll
+    for (int e = 0; e < V; ++e) s.b[e] = m[j][e] * i[j][e] * xs[j][e];
     if (starts(j)) {
-      const f32x2 h = initial(j);
-      s.b = f32x2{__builtin_fmaf(a[j].x, h.x, s.b.x), __builtin_fmaf(a[j].y, h.y, s.b.y)};
-      s.a = f32x2{0.f, 0.f};
+      s.b = apply<false>(s, initial(j));
+      s.a = vec_of<V>(0.f);
     }
     own = then<PACKED>(own, s);
   }
-  Step rev = no_step();
+  Step<V> rev = no_step<V>();
 #pragma unroll
   for (int j = R - 1; j >= 0; --j) {
-    const bool cut = ends(j);
-    const f32x2 g = cut ? d[j] : f32x2{rev.b.x + d[j].x, rev.b.y + d[j].y};
-    if (PACKED && !counts(j)) {
-      rev = Step{f32x2{0.f, 0.f}, f32x2{0.f, 0.f}};
-    } else {
-      rev.a = cut ? f32x2{0.f, 0.f} : factor<PACKED>(rev.a, a[j]);
-      rev.b = f32x2{a[j].x * g.x, a[j].y * g.y};
+    const bool cut = ends(j), out = PACKED && !counts(j);
+#pragma unroll
+    for (int e = 0; e < V; ++e) {
+      const float g = cut ? d[j][e] : rev.b[e] + d[j][e];
+      rev.a[e] = cut || out ? 0.f : factor1<PACKED>(rev.a[e], a[j][e]);
+      rev.b[e] = out ? 0.f : a[j][e] * g;
     }
   }
-  steps[wave][lane] = f32x4{own.a.x, own.a.y, own.b.x, own.b.y};
-  back[wave][lane] = f32x4{rev.a.x, rev.a.y, rev.b.x, rev.b.y};
+  steps.put(wave, lane, own);
+  back.put(wave, lane, rev);
   lds_barrier();
-  Step behind = no_step();
-  for (int w = NW - 1; w > wave; --w) {
-    const f32x4 s = back[w][lane];
-    behind = then<PACKED>(behind, Step{f32x2{s.x, s.y}, f32x2{s.z, s.w}});
-  }
-  if (wave == 0) leave_step(q, chain, n, cl, then<PACKED>(behind, rev));
-  f32x2 h = saved;
-  for (int w = 0; w < wave; ++w) {
-    const f32x4 s = steps[w][lane];
-    h = apply<PACKED>(Step{f32x2{s.x, s.y}, f32x2{s.z, s.w}}, h);
-  }
+  Step<V> behind = no_step<V>();
+  for (int w = NW - 1; w > wave; --w) behind = then<PACKED>(behind, back.get(w, lane));
+  if (wave == 0) leave_step(q, chain, n, lane, then<PACKED>(behind, rev));
+  for (int w = 0; w < wave; ++w) h = apply<PACKED>(steps.get(w, lane), h);
 #pragma unroll
   for (int j = 0; j < R; ++j) {
     if (starts(j)) h = initial(j);
-    if (PACKED && !counts(j)) h = f32x2{0.f, 0.f};
-    const f32x2 ix = {i[j].x * xs[j].x, i[j].y * xs[j].y};
-    f[j] = f32x2{a[j].x * __builtin_fmaf(a[j].x * ix.x, f[j].x, -r[j].x * h.x), a[j].y * __builtin_fmaf(a[j].y * ix.y, f[j].y, -r[j].y * h.y)};
-    h = f32x2{__builtin_fmaf(a[j].x, h.x, m[j].x * ix.x), __builtin_fmaf(a[j].y, h.y, m[j].y * ix.y)};
+    if (PACKED && !counts(j)) h = vec_of<V>(0.f);
+#pragma unroll
+    for (int e = 0; e < V; ++e) {
+      const float ix = i[j][e] * xs[j][e];
+      f[j][e] = a[j][e] * __builtin_fmaf(a[j][e] * ix, f[j][e], -r[j][e] * h[e]);
+      h[e] = __builtin_fmaf(a[j][e], h[e], m[j][e] * ix);
+    }
   }
   if (wave == NW - 1) {
-    f32x2 first = {0.f, 0.f};
-    if (!PACKED && p.dfinal_states) first = at.load_state(p.dfinal_states + (int64_t)b * p.dim, c);
-    enter[lane] = entering<PACKED>(q, chain, n, cl, first);
+    Vec<V> first = vec_of<V>(0.f);
+    if (!PACKED && p.dfinal_states) first = at.load_state(p.dfinal_states + (int64_t)b * p.dim);
+    enter[lane] = entering<PACKED>(q, chain, n, lane, first);
   }
   lds_barrier();
-  f32x2 carry = apply<PACKED>(behind, enter[lane]), sum = {0.f, 0.f};
-  if (wave == 0) leave_state(q, chain, n, cl, apply<PACKED>(rev, carry));
+  Vec<V> carry = apply<PACKED>(behind, enter[lane]), sum = vec_of<V>(0.f);
+  if (wave == 0) leave_state(q, chain, n, lane, apply<PACKED>(rev, carry));
   T *dxp = static_cast<T *>(p.dx) + b * p.dx_bs;
   T *dap = static_cast<T *>(p.dgate_a) + b * p.dgate_a_bs;
   T *dgp = static_cast<T *>(p.dgate_x) + b * p.dgate_x_bs;
 #pragma unroll
   for (int j = R - 1; j >= 0; --j) {
-    f32x2 g = ends(j) ? d[j] : f32x2{d[j].x + carry.x, d[j].y + carry.y};
-    if (PACKED && !counts(j)) g = f32x2{0.f, 0.f};
-    const int64_t t = t0 + j;
-    const f32x2 e = {g.x * f[j].x, g.y * f[j].y}, dx = {g.x * m[j].x * i[j].x, g.y * m[j].y * i[j].y};
-    if (j < rows) {
-      at.store(dxp + t * p.dx_ls, c, dx.x, dx.y);
-      at.store(dap + t * p.dgate_a_ls, c, k0 * (1.f - r[j].x) * e.x, k1 * (1.f - r[j].y) * e.y);
-      at.store(dgp + t * p.dgate_x_ls, c, dx.x * xs[j].x * (1.f - i[j].x), dx.y * xs[j].y * (1.f - i[j].y));
+    Vec<V> dx, da, dg;
+#pragma unroll
+    for (int e = 0; e < V; ++e) {
+      float g = ends(j) ? d[j][e] : d[j][e] + carry[e];
+      if (PACKED && !counts(j)) g = 0.f;
+      const float ee = g * f[j][e];
+      dx[e] = g * m[j][e] * i[j][e];
+      da[e] = rate.k[e] * (1.f - r[j][e]) * ee;
+      dg[e] = dx[e] * xs[j][e] * (1.f - i[j][e]);
+      if (counts(j)) sum[e] += ee;
+      carry[e] = a[j][e] * g;
     }
-    if (counts(j)) sum = f32x2{sum.x + e.x, sum.y + e.y};
-    carry = f32x2{a[j].x * g.x, a[j].y * g.y};
-    if (starts(j) && p.dinitial_states) at.store_state(p.dinitial_states + (int64_t)rowsof.seq[PACKED ? j : 0] * p.dim, c, carry);
+    if (j < rows) {
+      const int64_t t = t0 + j;
+      at.store(dxp + t * p.dx_ls, dx);
+      at.store(dap + t * p.dgate_a_ls, da);
+      at.store(dgp + t * p.dgate_x_ls, dg);
+    }
+    if (starts(j) && p.dinitial_states) at.store_state(p.dinitial_states + state_of(j), carry);
   }
-  if (!PACKED && t0 == 0 && p.dinitial_states) at.store_state(p.dinitial_states + (int64_t)b * p.dim, c, carry);
+  if (!PACKED && t0 == 0 && p.dinitial_states) at.store_state(p.dinitial_states + (int64_t)b * p.dim, carry);
   if constexpr (PACKED) {
     if (p.dinitial_states && tile == 0)
       empty_sequences(p.cu_seqlens, p.nseq, L, [&](int s) {
         const int64_t o = (int64_t)s * p.dim;
-        at.store_state(p.dinitial_states + o, c, p.dfinal_states ? at.load_state(p.dfinal_states + o, c) : f32x2{0.f, 0.f});
+        at.store_state(p.dinitial_states + o, p.dfinal_states ? at.load_state(p.dfinal_states + o) : vec_of<V>(0.f));
       });
   }
   // the terms of ddecay over the tile (the steps were read before the last barrier)
-  f32x2 *sums = reinterpret_cast<f32x2 *>(&steps[0][0]);
-  sums[wave * 64 + lane] = sum;
+  steps.put(wave, lane, Step<V>{sum, sum});
   lds_barrier();
   if (wave == 0) {
+    for (int w = 1; w < NW; ++w) {
+      const Vec<V> s = steps.get(w, lane).a;
 #pragma unroll
-    for (int w = 1; w < NW; ++w) sum = f32x2{sum.x + sums[w * 64 + lane].x, sum.y + sums[w * 64 + lane].y};
-    const f32x2 slope = {p.rate / (1.f + expf(-d0)), p.rate / (1.f + expf(-d1))};
-    at.store_state(parts + ((int64_t)b * q.ntiles + tile) * p.dim, c, f32x2{sum.x * slope.x, sum.y * slope.y});
+      for (int e = 0; e < V; ++e) sum[e] += s[e];
+    }
+#pragma unroll
+    for (int e = 0; e < V; ++e) sum[e] *= p.rate / (1.f + expf(-rate.d[e]));
+    at.store_state(parts + ((int64_t)b * q.ntiles + tile) * p.dim, sum);
   }
 }
 
 // ------------------------------------------------------------------ host side
-constexpr int kFwdRows = 8, kFwdWaves = 8, kBwdRows = 4, kBwdWaves = 8;
+constexpr int kV = 2, kFwdRows = 16, kFwdWaves = 4, kBwdRows = 4, kBwdWaves = 8, kGroup = 8;
+constexpr int kTileChannels = 64 * kV;
 
 // Tiles of one pass and what its chains need in memory: the tickets and words, cleared before the launch, lie at the
 // start of the buffer, `tail` behind them.
@@ -258,7 +284,7 @@ struct Plan {
   }
   static int group_of(int64_t chains, int ntiles) {
     (void)chains;
-    return min(ntiles, 8);
+    return min(ntiles, kGroup);
   }
   Chain chain(void *buf) const {
     Chain q;
@@ -295,7 +321,7 @@ int check(const GatedScanParams *p, bool bwd) {
 // f(T{}, even, packed) with the call's types as compile-time values
 template <typename F> int with_forms(const GatedScanParams &p, F f) {
   auto forms = [&](auto t) {
-    const bool even = p.dim % 2 == 0;
+    const bool even = p.dim % kV == 0;
     if (p.nseq > 0) return even ? f(t, std::true_type{}, std::true_type{}) : f(t, std::false_type{}, std::true_type{});
     return even ? f(t, std::true_type{}, std::false_type{}) : f(t, std::false_type{}, std::false_type{});
   };
@@ -326,7 +352,7 @@ extern "C" int gated_scan_fwd(const GatedScanParams *p, mamba_stream_t stream) {
     if (const int rc = mamba_hip_zero(p->ckpt, plan.head, stream)) return rc;
   float *ck = reinterpret_cast<float *>(static_cast<char *>(p->ckpt) + plan.head);
   return with_forms(*p, [&](auto t, auto even, auto packed) {
-    gated_fwd_kernel<decltype(t), even.value, packed.value, kFwdRows, kFwdWaves>
+    gated_fwd_kernel<decltype(t), kV, even.value, packed.value, kFwdRows, kFwdWaves>
         <<<dim3((unsigned)(plan.chains * plan.ntiles)), dim3(kFwdWaves * 64), 0, static_cast<hipStream_t>(stream)>>>(
             *p, plan.chain(p->ckpt), ck, kBwdRows * kBwdWaves, bwd_plan(*p).ntiles);
     return hipGetLastError() == hipSuccess ? MAMBA_OK : MAMBA_E_LAUNCH;
@@ -341,7 +367,7 @@ extern "C" int gated_scan_bwd(const GatedScanParams *p, mamba_stream_t stream) {
   const float *ck = reinterpret_cast<const float *>(static_cast<const char *>(p->ckpt) + fwd_plan(*p).head);
   float *parts = reinterpret_cast<float *>(static_cast<char *>(p->ws) + plan.head);
   const int rc = with_forms(*p, [&](auto t, auto even, auto packed) {
-    gated_bwd_kernel<decltype(t), even.value, packed.value, kBwdRows, kBwdWaves>
+    gated_bwd_kernel<decltype(t), kV, even.value, packed.value, kBwdRows, kBwdWaves>
         <<<dim3((unsigned)(plan.chains * plan.ntiles)), dim3(kBwdWaves * 64), 0, st>>>(*p, plan.chain(p->ws), ck, parts);
     return hipGetLastError() == hipSuccess ? MAMBA_OK : MAMBA_E_LAUNCH;
   });

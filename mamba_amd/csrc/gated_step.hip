@@ -21,8 +21,8 @@ __global__ __launch_bounds__(256) void gated_step_kernel(const GatedStepParams p
   S *sp = static_cast<S *>(p.state) + row * p.state_rs + c;
   for (int e = 0; e < n; ++e) {
     const float k = p.rate * softplus_exact(ld_param(p.decay, p.decay_dtype, c + e));
-    const Gates q(ld1<T>(ap + e), ld1<T>(gp + e), k);
-    const float h = __builtin_fmaf(q.a, ld1<S>(sp + e), q.m * q.i * ld1<T>(xp + e));
+    const Gates q(ld1<T>(ap + e), ld1<T>(gp + e), k, -k * kLog2e);
+    const float h = __builtin_fmaf(q.a, ld1<S>(sp + e), q.m() * q.i * ld1<T>(xp + e));
     st1<S>(sp + e, h);
     st1<T>(op + e, h);
   }

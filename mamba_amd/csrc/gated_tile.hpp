@@ -1,97 +1,141 @@
 // Tiles of the gated linear recurrence: what the forward and the backward kernel of gated_scan.hip share.
 //
 // A row of positions is a linear recurrence per channel, h = a h + b, and a run of positions is one such step (A, B)
-// again.  The row is cut into tiles of positions and groups of 128 channels.  A workgroup holds one tile of one group
-// in registers: a wave has ROWS positions after one another, its lanes two channels each (rows of 256 or 512 bytes).
-// The steps of the waves meet in LDS; the state that enters the tile comes from the workgroups of the tiles before it
-// (`Chain`), so every tensor is read once and written once.
+// again.  The row is cut into tiles of positions and groups of 64 V channels.  A workgroup holds one tile of one group
+// in registers: a wave has R positions after one another, its lanes V channels each.  The steps of the waves meet in
+// LDS; the state that enters the tile comes from the workgroups of the tiles before it (`Chain`), so every tensor is
+// read once and written once.
 #pragma once
 #include "gated_gates.hpp"
 
 namespace {
 
-constexpr int kTileChannels = 128;
-
-// Two neighbouring channels of one position.
-template <typename T> struct Pair {
-  uint32_t w;
-  DEVI float lo() const { return DT<T>::id == MAMBA_BF16 ? bf16_lo(w) : f16_lo(w); }
-  DEVI float hi() const { return DT<T>::id == MAMBA_BF16 ? bf16_hi(w) : f16_hi(w); }
+template <int V> struct Vec {
+  float v[V];
+  DEVI float &operator[](int e) { return v[e]; }
+  DEVI const float &operator[](int e) const { return v[e]; }
 };
-template <> struct Pair<float> {
-  u32x2 w;
-  DEVI float lo() const { return __builtin_bit_cast(f32x2, w).x; }
-  DEVI float hi() const { return __builtin_bit_cast(f32x2, w).y; }
+template <int V> DEVI Vec<V> vec_of(float x) {
+  Vec<V> r;
+#pragma unroll
+  for (int e = 0; e < V; ++e) r[e] = x;
+  return r;
+}
+
+// W words that lie at the alignment of a 2- or 4-byte element.
+template <int W, int A> struct Words;
+template <int W> struct Words<W, 2> {
+  typedef uint32_t type __attribute__((ext_vector_type(W), aligned(2)));
+};
+template <int W> struct Words<W, 4> {
+  typedef uint32_t type __attribute__((ext_vector_type(W), aligned(4)));
 };
 
-// How a lane reads and writes its pair of channels c, c + 1.  EVEN: the number of channels is even, a pair is whole or
-// not there.  Otherwise the last channel may stand alone: the lane reads the pair before it and takes its second half.
-// Rows lie at any alignment (gfx950 serves these accesses at element alignment).  Lanes past the last channel read
-// the last pair again and write nothing.
-template <typename T, bool EVEN> struct Lane {
-  int at;         // the channel that the lane's pair is read from
-  bool two, one;  // whether both channels, or the first alone, are there
-  bool half;      // the pair holds the first channel in its second half
-  bool single;    // a row of one channel
-  DEVI Lane(int c, int dim) {
-    two = c + 1 < dim;
-    one = !EVEN && c + 1 == dim;
-    at = max(min(c, dim - 2), 0);
-    half = !EVEN && c > dim - 2;
-    single = !EVEN && dim == 1;
+// V neighbouring channels of one position as they lie in memory.
+template <typename T, int V> struct Raw {
+  static constexpr int W = V * (DT<T>::id == MAMBA_F32 ? 4 : 2) / 4;
+  uint32_t w[W];
+  DEVI float get(int e) const {
+    if constexpr (DT<T>::id == MAMBA_F32) return __builtin_bit_cast(float, w[e]);
+    else if constexpr (DT<T>::id == MAMBA_BF16) return e & 1 ? bf16_hi(w[e / 2]) : bf16_lo(w[e / 2]);
+    else return e & 1 ? f16_hi(w[e / 2]) : f16_lo(w[e / 2]);
   }
-  DEVI Pair<T> load(const T *row) const {
-    Pair<T> r;
-    if constexpr (DT<T>::id == MAMBA_F32) {
-      typedef u32x2 a4 __attribute__((aligned(4)));
-      if (!EVEN && single) {
-        r.w = u32x2{*(const GLOBAL_AS uint32_t *)row, 0u};
-        return r;
+};
+
+// How a lane reads and writes its channels c .. c + V - 1.  WHOLE: the number of channels is a multiple of V, all of a
+// lane's channels are there or none.  Otherwise a lane at the end reads the last V channels and moves its own to the
+// front.  Rows lie at any alignment (gfx950 serves these accesses at element alignment).  Lanes past the last channel
+// read the last ones again and write nothing.
+template <typename T, int V, bool WHOLE> struct Lane {
+  static constexpr int W = Raw<T, V>::W;
+  int c, n;         // the lane's first channel, how many of its channels are there
+  int dim, shift;   // the channel read first lies `shift` before c
+  uint32_t at, to;  // byte offsets in a row: of what is read, of c
+  DEVI Lane(int c_, int dim_) : c(c_), dim(dim_) {
+    n = min(max(dim - c, 0), V);
+    const int from = max(min(c, dim - V), 0);
+    shift = min(c - from, V - 1);
+    at = (uint32_t)from * sizeof(T);
+    to = (uint32_t)c * sizeof(T);
+  }
+  DEVI Raw<T, V> load(const T *row) const {
+    Raw<T, V> r;
+    const GLOBAL_AS char *p = (const GLOBAL_AS char *)row;
+    if (!WHOLE && dim < V) {  // fewer channels in a row than a lane holds
+      uint32_t q[V];
+#pragma unroll
+      for (int e = 0; e < V; ++e) {
+        const uint32_t o = (uint32_t)min(e, dim - 1) * sizeof(T);
+        if constexpr (sizeof(T) == 4) q[e] = *(const GLOBAL_AS uint32_t *)(p + o);
+        else q[e] = *(const GLOBAL_AS uint16_t *)(p + o);
       }
-      r.w = *(const GLOBAL_AS a4 *)(row + at);
-      if (!EVEN) r.w.x = half ? r.w.y : r.w.x;
-    } else {
-      typedef uint32_t a2 __attribute__((aligned(2)));
-      if (!EVEN && single) {
-        r.w = *(const GLOBAL_AS uint16_t *)row;
-        return r;
+#pragma unroll
+      for (int e = 0; e < V; ++e) {
+        if constexpr (sizeof(T) == 4) r.w[e] = q[e];
+        else if (e & 1) r.w[e / 2] = q[e - 1] | q[e] << 16;
       }
-      r.w = *(const GLOBAL_AS a2 *)(row + at);
-      if (!EVEN) r.w = half ? r.w >> 16 : r.w;
+      return r;
+    }
+    typedef typename Words<W, sizeof(T)>::type words;
+    const words v = *(const GLOBAL_AS words *)(p + at);
+#pragma unroll
+    for (int i = 0; i < W; ++i) r.w[i] = v[i];
+    if constexpr (!WHOLE) {
+#pragma unroll
+      for (int step = V / 2; step >= 1; step >>= 1) {  // move by `step` channels where shift says so
+        const bool on = shift & step;
+#pragma unroll
+        for (int i = 0; i < W; ++i) {
+          uint32_t up;
+          if constexpr (sizeof(T) == 4) up = i + step < W ? r.w[i + step] : 0u;
+          else if (step >= 2) up = i + step / 2 < W ? r.w[i + step / 2] : 0u;
+          else up = r.w[i] >> 16 | (i + 1 < W ? r.w[i + 1] << 16 : 0u);
+          r.w[i] = on ? up : r.w[i];
+        }
+      }
     }
     return r;
   }
-  DEVI void store(T *row, int c, float lo, float hi) const {
-    if (two) {
-      if constexpr (DT<T>::id == MAMBA_F32) {
-        typedef f32x2 a4 __attribute__((aligned(4)));
-        *(GLOBAL_AS a4 *)(row + c) = f32x2{lo, hi};
-      } else {
-        typedef uint32_t a2 __attribute__((aligned(2)));
-        *(GLOBAL_AS a2 *)(row + c) = DT<T>::id == MAMBA_BF16 ? pack_bf16(lo, hi) : pack_f16(lo, hi);
+  DEVI void store(T *row, const Vec<V> &x) const {
+    typedef typename Words<W, sizeof(T)>::type words;
+    GLOBAL_AS char *p = (GLOBAL_AS char *)row + to;
+    if (n == V) {
+      words v;
+#pragma unroll
+      for (int i = 0; i < W; ++i) {
+        if constexpr (DT<T>::id == MAMBA_F32) v[i] = __builtin_bit_cast(uint32_t, x.v[i]);
+        else if constexpr (DT<T>::id == MAMBA_BF16) v[i] = pack_bf16(x.v[2 * i], x.v[2 * i + 1]);
+        else v[i] = pack_f16(x.v[2 * i], x.v[2 * i + 1]);
       }
-    } else if (!EVEN && one) {
-      st1<T>(row + c, lo);
+      *(GLOBAL_AS words *)p = v;
+    } else if (!WHOLE) {
+#pragma unroll
+      for (int e = 0; e < V; ++e)
+        if (e < n) st1<T>(row + c + e, x[e]);
     }
   }
-  DEVI f32x2 load_state(const float *row, int c) const {
-    return f32x2{two || one ? row[c] : 0.f, two ? row[c + 1] : 0.f};
+  DEVI Vec<V> load_state(const float *row) const {
+    Vec<V> r;
+#pragma unroll
+    for (int e = 0; e < V; ++e) r[e] = e < n ? row[c + e] : 0.f;
+    return r;
   }
-  DEVI void store_state(float *row, int c, f32x2 v) const {
-    if (two || one) row[c] = v.x;
-    if (two) row[c + 1] = v.y;
+  DEVI void store_state(float *row, const Vec<V> &x) const {
+#pragma unroll
+    for (int e = 0; e < V; ++e)
+      if (e < n) row[c + e] = x[e];
   }
 };
 
-// The step of a run of positions for two channels: h -> a h + b.
-struct Step {
-  f32x2 a, b;
-};
-DEVI Step no_step() { return Step{f32x2{1.f, 1.f}, f32x2{0.f, 0.f}}; }
+// The step of a run of positions: h -> a h + b per channel.
 // RESETS: a factor of exactly 0 marks a run in which a sequence starts; nothing before it counts, whatever it is.  The
 // decays of positions are kept from underflowing to that (a state times kTiny is gone all the same, but an infinity or a
 // NaN in the sequence stays one).
 constexpr float kTiny = 1.17549435e-38f;
+template <int V> struct Step {
+  Vec<V> a, b;
+};
+template <int V> DEVI Step<V> no_step() { return Step<V>{vec_of<V>(1.f), vec_of<V>(0.f)}; }
 template <bool RESETS> DEVI float apply1(float a, float b, float h) {
   const float r = __builtin_fmaf(a, h, b);
   return RESETS && a == 0.f ? b : r;
@@ -101,15 +145,38 @@ template <bool RESETS> DEVI float factor1(float a, float next) {
   if (!RESETS) return r;
   return a == 0.f || next == 0.f ? 0.f : fmaxf(r, kTiny);
 }
-template <bool RESETS> DEVI f32x2 apply(const Step &s, f32x2 h) {
-  return f32x2{apply1<RESETS>(s.a.x, s.b.x, h.x), apply1<RESETS>(s.a.y, s.b.y, h.y)};
+template <bool RESETS, int V> DEVI Vec<V> apply(const Step<V> &s, const Vec<V> &h) {
+  Vec<V> r;
+#pragma unroll
+  for (int e = 0; e < V; ++e) r[e] = apply1<RESETS>(s.a[e], s.b[e], h[e]);
+  return r;
 }
-template <bool RESETS> DEVI f32x2 factor(f32x2 a, f32x2 next) {
-  return f32x2{factor1<RESETS>(a.x, next.x), factor1<RESETS>(a.y, next.y)};
+template <bool RESETS, int V> DEVI Step<V> then(const Step<V> &s, const Step<V> &next) {
+  Step<V> r;
+#pragma unroll
+  for (int e = 0; e < V; ++e) r.a[e] = factor1<RESETS>(s.a[e], next.a[e]);
+  r.b = apply<RESETS>(next, s.b);
+  return r;
 }
-template <bool RESETS> DEVI Step then(const Step &s, const Step &next) {
-  return Step{factor<RESETS>(s.a, next.a), apply<RESETS>(next, s.b)};
-}
+
+// The steps of a workgroup's waves in LDS.
+template <int V, int NW> struct WaveSteps {
+  typedef float fvec __attribute__((ext_vector_type(V)));
+  fvec a[NW][64], b[NW][64];
+  DEVI void put(int wave, int lane, const Step<V> &s) {
+    fvec x, y;
+#pragma unroll
+    for (int e = 0; e < V; ++e) x[e] = s.a[e], y[e] = s.b[e];
+    a[wave][lane] = x, b[wave][lane] = y;
+  }
+  DEVI Step<V> get(int wave, int lane) const {
+    const fvec x = a[wave][lane], y = b[wave][lane];
+    Step<V> s;
+#pragma unroll
+    for (int e = 0; e < V; ++e) s.a[e] = x[e], s.b[e] = y[e];
+    return s;
+  }
+};
 
 // How the tiles of one row and channel group hand the state on, always in the same order of additions.  `group` tiles
 // form a group: a tile reads the steps of the tiles before it in its group and the state at the end of the group before,
@@ -121,8 +188,8 @@ template <bool RESETS> DEVI Step then(const Step &s, const Step &next) {
 // are started.
 struct Chain {
   uint32_t *tickets;  // one per chain (row and channel group)
-  uint64_t *steps;    // (chain, ntiles, 128)
-  uint64_t *states;   // (chain, ngroups, 128)
+  uint64_t *steps;    // (chain, ntiles, 64 V)
+  uint64_t *states;   // (chain, ngroups, 64 V)
   int ntiles, group, ngroups;
 };
 constexpr uint64_t kThere = 1ull << 63;
@@ -132,64 +199,67 @@ DEVI uint64_t word_of(float a, float b) {
 }
 DEVI float word_a(uint64_t w) { return __builtin_bit_cast(float, (uint32_t)(w >> 32) & 0x7fffffffu); }
 DEVI float word_b(uint64_t w) { return __builtin_bit_cast(float, (uint32_t)w); }
-DEVI void put_words(uint64_t *p, f32x2 a, f32x2 b) {
-  __hip_atomic_store(p, word_of(a.x, b.x), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-  __hip_atomic_store(p + 1, word_of(a.y, b.y), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+template <int V> DEVI void put_words(uint64_t *p, const Step<V> &s) {
+#pragma unroll
+  for (int e = 0; e < V; ++e) __hip_atomic_store(p + e, word_of(s.a[e], s.b[e]), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
-DEVI uint64_t get_word(const uint64_t *p) { return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
 
-// Whole wave: the two words of every lane for N tiles, `stride` words apart, once all of them are there.
-template <int N> DEVI void wait_words(const uint64_t *p, int64_t stride, uint64_t (&w)[N][2]) {
+// Whole wave: the words of every lane for N tiles, 64 V words apart, once all of them are there.
+template <int V, int N> DEVI void wait_words(const uint64_t *p, uint64_t (&w)[N][V]) {
   for (;;) {
-    bool there = true;
+    uint64_t all = kThere;
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
-      w[i][0] = get_word(p + i * stride);
-      w[i][1] = get_word(p + i * stride + 1);
-    }
+    for (int i = 0; i < N; ++i)
 #pragma unroll
-    for (int i = 0; i < N; ++i) there = there && (w[i][0] & w[i][1] & kThere) != 0;
-    if (__all(there)) return;
+      for (int e = 0; e < V; ++e) w[i][e] = __hip_atomic_load(p + i * 64 * V + e, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+#pragma unroll
+      for (int e = 0; e < V; ++e) all &= w[i][e];
+    if (__all(all != 0)) return;
     __builtin_amdgcn_s_sleep(1);
   }
 }
 
-// Whole wave: the state that enters tile n of the chain; `first` is the one that enters tile 0.  c: the lane's place in the
-// channel group (0, 2, .. 126).
-template <bool RESETS> DEVI f32x2 entering(const Chain &q, int64_t chain, int n, int c, f32x2 first) {
-  const int g = n / q.group, from = g * q.group;
-  const uint64_t *sp = q.steps + (chain * q.ntiles + from) * kTileChannels + c;
-  Step s = no_step();
+// Whole wave: the state that enters tile n of the chain; `first` is the one that enters tile 0.
+template <bool RESETS, int V> DEVI Vec<V> entering(const Chain &q, int64_t chain, int n, int lane, Vec<V> first) {
+  const int g = n / q.group, from = g * q.group, count = n - from;
+  const uint64_t *sp = q.steps + (chain * q.ntiles + from) * (64 * V) + lane * V;
+  Step<V> s = no_step<V>();
+  auto take = [&](const uint64_t (&w)[V]) {
+    Step<V> next;
+#pragma unroll
+    for (int e = 0; e < V; ++e) next.a[e] = word_a(w[e]), next.b[e] = word_b(w[e]);
+    s = then<RESETS>(s, next);
+  };
   int i = 0;
   constexpr int B = 4;
-  auto take = [&](const uint64_t (&w)[2]) {
-    s = then<RESETS>(s, Step{f32x2{word_a(w[0]), word_a(w[1])}, f32x2{word_b(w[0]), word_b(w[1])}});
-  };
-  for (; i + B <= n - from; i += B) {
-    uint64_t w[B][2];
-    wait_words<B>(sp + i * kTileChannels, kTileChannels, w);
+  for (; i + B <= count; i += B) {
+    uint64_t w[B][V];
+    wait_words<V, B>(sp + (int64_t)i * 64 * V, w);
 #pragma unroll
     for (int j = 0; j < B; ++j) take(w[j]);
   }
-  for (; i < n - from; ++i) {
-    uint64_t w[1][2];
-    wait_words<1>(sp + i * kTileChannels, kTileChannels, w);
+  for (; i < count; ++i) {
+    uint64_t w[1][V];
+    wait_words<V, 1>(sp + (int64_t)i * 64 * V, w);
     take(w[0]);
   }
   if (g > 0) {
-    uint64_t w[1][2];
-    wait_words<1>(q.states + (chain * q.ngroups + g - 1) * kTileChannels + c, 0, w);
-    first = f32x2{word_b(w[0][0]), word_b(w[0][1])};
+    uint64_t w[1][V];
+    wait_words<V, 1>(q.states + (chain * q.ngroups + g - 1) * (64 * V) + lane * V, w);
+#pragma unroll
+    for (int e = 0; e < V; ++e) first[e] = word_b(w[0][e]);
   }
   return apply<RESETS>(s, first);
 }
 // What tile n leaves for the ones behind it: its step at once, the state at its end where it closes a group.
-DEVI void leave_step(const Chain &q, int64_t chain, int n, int c, const Step &s) {
-  if (n + 1 < q.ntiles && (n + 1) % q.group != 0) put_words(q.steps + (chain * q.ntiles + n) * kTileChannels + c, s.a, s.b);
+template <int V> DEVI void leave_step(const Chain &q, int64_t chain, int n, int lane, const Step<V> &s) {
+  if (n + 1 < q.ntiles && (n + 1) % q.group != 0) put_words<V>(q.steps + (chain * q.ntiles + n) * (64 * V) + lane * V, s);
 }
-DEVI void leave_state(const Chain &q, int64_t chain, int n, int c, f32x2 h) {
+template <int V> DEVI void leave_state(const Chain &q, int64_t chain, int n, int lane, const Vec<V> &h) {
   if (n + 1 < q.ntiles && (n + 1) % q.group == 0)
-    put_words(q.states + (chain * q.ngroups + n / q.group) * kTileChannels + c, f32x2{0.f, 0.f}, h);
+    put_words<V>(q.states + (chain * q.ngroups + n / q.group) * (64 * V) + lane * V, Step<V>{vec_of<V>(0.f), h});
 }
 
 // The tile of this workgroup within its chain: the number of workgroups of the chain that began before it.  (lds: one int.)

@@ -152,13 +152,13 @@ inline int wide_threads(int channels) { return (channels / 8 + 63) / 64 * 64; }
 // workgroups of that many threads which a CU holds at once at `waves_per_simd` waves per SIMD
 inline int wide_resident(int threads, int waves_per_simd) { return max(1, waves_per_simd * 4 / (threads / 64)); }
 
-// Column sums of up to five (nparts, dim) workspaces, in the order of the parts, written in the parameters' dtype:
+// Column sums of up to four (nparts, dim) workspaces, in the order of the parts, written in the parameters' dtype:
 // blockIdx.y is the workspace, a workgroup takes 16 channels (64 bytes of every row) on 128 slices of the parts, four
 // of a thread's rows in flight.  (64 channels x 16 slices of 1024 threads took 25 us for 1024 parts of 2560 channels:
 // 40 workgroups, one row at a time per thread.)
 struct ReduceJobs {
-  const float *part[5];
-  void *out[5];
+  const float *part[4];
+  void *out[4];
 };
 template <bool VEC> __global__ __launch_bounds__(512) void norm_reduce_kernel(const ReduceJobs jobs, int dtype, int nparts, int dim) {
   constexpr int SLICES = 128;

@@ -4,7 +4,8 @@
 // device guard, done on at::Tensor, so that one call costs a few microseconds of host time instead of the ~15 us the
 // same work takes in Python + ctypes; and the operators' autograd nodes, whose backward passes then run without the
 // interpreter.  This file has the decode-step operators and the module; torch_norm_conv.cpp the norms and the
-// convolution, torch_scan.cpp and torch_ssd.cpp the training operators and the mixers built on them.
+// convolution, torch_scan.cpp and torch_ssd.cpp the training operators and the mixers built on them,
+// torch_gated.cpp the gated linear recurrence and the norm between two blocks.
 // Built as the Python extension module mamba_amd._torch_ext (pybind11), linked against
 // libmamba_gfx950.so; it contains no device code.
 #include "torch_common.h"
@@ -202,4 +203,5 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   bind_norm_conv(m);
   bind_scan(m);
   bind_ssd(m);
+  bind_gated(m);
 }

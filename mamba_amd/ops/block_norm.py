@@ -85,7 +85,8 @@ class BlockNormFn(torch.autograd.Function):
             with torch.cuda.device(x.device):
                 lib = _lib.load()
                 p.nparts = lib.norm_block_bwd_nparts(p)
-                parts = torch.empty(len(given), p.nparts, dim, dtype=torch.float32, device=x.device)
+                nsums = 2 + (norm_bias is not None) + (next_bias is not None)
+                parts = torch.empty(nsums, p.nparts, dim, dtype=torch.float32, device=x.device)
                 p.parts = parts.data_ptr()
                 _lib.check(lib.norm_block_bwd(p, _lib.current_stream(x.device)), "norm_block_bwd")
         og = lambda t: t.reshape(ctx.shape) if t is not None else None
@@ -109,8 +110,15 @@ def block_norm_fn(x, residual, norm_weight, next_weight, z=None, scale=None, nor
     Return:
         out in x's dtype, residual_out in residual's (the sum is normed before it is rounded to that)
     """
-    what = "block_norm"
     tensor_scale = scale if isinstance(scale, torch.Tensor) else None
+    number = 1.0 if scale is None or tensor_scale is not None else float(scale)
+    ext = _lib.torch_ext()
+    if ext is not None:
+        # the same node in C++ (csrc/torch_gated.cpp); None = a case for the code below
+        r = ext.block_norm(x, residual, norm_weight, next_weight, z, tensor_scale, number, norm_bias, next_bias, eps, bool(is_rms_norm))
+        if r is not None:
+            return r
+    what = "block_norm"
     if x.dim() < 1 or x.dtype not in _lib.DTYPE_CODE:
         raise RuntimeError(f"{what}: x must be (..., dim) in fp32, fp16 or bf16")
     for name, t in (("residual", residual), ("z", z)):
@@ -129,12 +137,10 @@ def block_norm_fn(x, residual, norm_weight, next_weight, z=None, scale=None, nor
     for t in (residual, z, *params.values()):
         if t is not None and t.device != x.device:
             raise RuntimeError(f"{what}: all tensors must be on {x.device}, got one on {t.device}")
-    if tensor_scale is None:
-        scale = 1.0 if scale is None else float(scale)
     one = len({t.dtype for t in params.values() if t is not None}) == 1
     conv = lambda t: None if t is None else (t if one else t.float()).contiguous()
     return BlockNormFn.apply(x, residual, conv(norm_weight), conv(next_weight), z.to(x.dtype) if z is not None else None,
-                             conv(scale) if tensor_scale is not None else scale, conv(norm_bias), conv(next_bias), float(eps),
+                             conv(scale) if tensor_scale is not None else number, conv(norm_bias), conv(next_bias), float(eps),
                              bool(is_rms_norm))
 
 

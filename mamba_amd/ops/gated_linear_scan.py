@@ -134,6 +134,12 @@ def gated_linear_scan_fn(x, gate_a, gate_x, decay, rate=8.0, initial_states=None
         out: (batch, seqlen, dim) in x's dtype, and with return_final_states also the states after the last positions,
         fp32, of initial_states' shape
     """
+    ext = _lib.torch_ext()
+    if ext is not None:
+        # the same checks, node and launches in C++ (csrc/torch_gated.cpp); None = a case for the code below
+        r = ext.gated_linear_scan(x, gate_a, gate_x, decay, rate, initial_states, cu_seqlens, bool(return_final_states))
+        if r is not None:
+            return r
     what = "gated_linear_scan"
     if x.dim() != 3 or x.dtype not in _lib.DTYPE_CODE:
         raise RuntimeError(f"{what}: x must be (batch, seqlen, dim) in fp32, fp16 or bf16")
@@ -175,6 +181,11 @@ def gated_linear_state_update(state, x, gate_a, gate_x, decay, rate=8.0, state_b
     Return:
         out: (batch, dim) in x's dtype, the new states
     """
+    ext = _lib.torch_ext()
+    if ext is not None:
+        out = ext.gated_linear_state_update(state, x, gate_a, gate_x, decay, rate, state_batch_indices)
+        if out is not None:
+            return out
     what = "gated_linear_state_update"
     if x.dim() != 2 or state.dim() != 2 or state.shape[1] != x.shape[1]:
         raise RuntimeError(f"{what}: state must be (rows, dim) and x (batch, dim)")
