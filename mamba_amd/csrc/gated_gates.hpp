@@ -4,14 +4,19 @@
 
 namespace {
 
-// softplus and its slope to the last bits: once per channel, not per position.  (An error in k repeats at every
-// position, and a long memory adds it up; softplus_f's 2e-6 near e^x = 0.05 would show in fp32 results.)
-DEVI float softplus_exact(float x) { return x > 20.f ? x : log1pf(expf(x)); }
-template <typename P> DEVI float decay_rate(const P &p, int c) {
-  return p.rate * softplus_exact(ld_param(p.decay, p.decay_dtype, c));
-}
-template <typename P> DEVI float decay_slope(const P &p, int c) {  // dk / ddecay
-  return p.rate / (1.f + expf(-ld_param(p.decay, p.decay_dtype, c)));
+// softplus to 2e-7 of its value at every size.  (An error in k repeats at every position, and a long memory adds it up;
+// softplus_f's 2e-6 near e^x = 0.05 would show in fp32 results.)  e = exp(x) with the rounding of its argument made good;
+// log(1 + e) = 2 atanh(e / (2 + e)) by its series below e = 0.5 (next term 1e-8 of the sum), the logarithm beyond.
+DEVI float softplus_exact(float x) {
+  const float t = x * kLog2e, lo = __builtin_fmaf(x, kLog2e, -t) + x * 1.9259629911e-8f;  // log2(e) = kLog2e + 1.93e-8
+  const float e = __builtin_amdgcn_exp2f(t) * __builtin_fmaf(lo, kLn2, 1.f);
+  const float s = e * fast_rcp(2.f + e), s2 = s * s;
+  float q = __builtin_fmaf(s2, 1.f / 9.f, 1.f / 7.f);
+  q = __builtin_fmaf(s2, q, 1.f / 5.f);
+  q = __builtin_fmaf(s2, q, 1.f / 3.f);
+  q = __builtin_fmaf(s2, q, 1.f);
+  const float r = e < 0.5f ? 2.f * s * q : fast_log(1.f + e);
+  return x <= 20.f ? r : x;
 }
 
 // One position's gates from kr's factor k and k2 = -k log2(e): r, i, a and m^2 = 1 - a^2.

@@ -1,35 +1,49 @@
 // One position of the gated linear recurrence (gated_scan.hip has the formulas), the states updated in place (gfx950).
-#include "gated_gates.hpp"
+// Every operand is read once and the state and output written once.  A thread has 4 channels of one batch entry, all its
+// loads in flight together; many short waves fill the memory's channels.
+#include "gated_tile.hpp"
+
+#include <type_traits>
 
 namespace {
 
-// V channels per thread; blockIdx.y is the batch entry.
-template <typename T, typename S, int V, bool VEC>
-__global__ __launch_bounds__(256) void gated_step_kernel(const GatedStepParams p) {
-  const int c = (blockIdx.x * 256 + threadIdx.x) * V, b = blockIdx.y;
+constexpr int kV = 4, kThreads = 256;
+
+template <typename T, typename S, bool WHOLE> __global__ __launch_bounds__(kThreads) void gated_step_kernel(const GatedStepParams p) {
+  const int c = (blockIdx.x * kThreads + threadIdx.x) * kV;
   if (c >= p.dim) return;
-  const int row = p.state_batch_indices ? p.state_batch_indices[b] : b;
-  T *op = static_cast<T *>(p.out) + b * p.out_rs + c;
-  const int n = min(V, p.dim - c);
-  if (row < 0 || row >= p.state_rows) {
-    for (int e = 0; e < n; ++e) st1<T>(op + e, 0.f);
-    return;
-  }
-  const T *xp = static_cast<const T *>(p.x) + b * p.x_rs + c;
-  const T *ap = static_cast<const T *>(p.gate_a) + b * p.gate_a_rs + c;
-  const T *gp = static_cast<const T *>(p.gate_x) + b * p.gate_x_rs + c;
-  S *sp = static_cast<S *>(p.state) + row * p.state_rs + c;
-  for (int e = 0; e < n; ++e) {
-    const float k = p.rate * softplus_exact(ld_param(p.decay, p.decay_dtype, c + e));
-    const Gates q(ld1<T>(ap + e), ld1<T>(gp + e), k, -k * kLog2e);
-    const float h = __builtin_fmaf(q.a, ld1<S>(sp + e), q.m() * q.i * ld1<T>(xp + e));
-    st1<S>(sp + e, h);
-    st1<T>(op + e, h);
+  const Lane<T, kV, WHOLE> at(c, p.dim);
+  const Lane<S, kV, WHOLE> st(c, p.dim);
+  for (int b = blockIdx.y; b < p.batch; b += gridDim.y) {
+    const int row = p.state_batch_indices ? p.state_batch_indices[b] : b;
+    T *out = static_cast<T *>(p.out) + b * p.out_rs;
+    if (row < 0 || row >= p.state_rows) {
+      at.store(out, vec_of<kV>(0.f));
+      continue;
+    }
+    S *state = static_cast<S *>(p.state) + row * p.state_rs;
+    const Raw<T, kV> ga = at.load(static_cast<const T *>(p.gate_a) + b * p.gate_a_rs);
+    const Raw<T, kV> gx = at.load(static_cast<const T *>(p.gate_x) + b * p.gate_x_rs);
+    const Raw<T, kV> x = at.load(static_cast<const T *>(p.x) + b * p.x_rs);
+    const Raw<S, kV> before = st.load(state);
+    Vec<kV> d, h;
+#pragma unroll
+    for (int e = 0; e < kV; ++e) d[e] = ld_param(p.decay, p.decay_dtype, min(c + e, p.dim - 1));
+#pragma unroll
+    for (int e = 0; e < kV; ++e) {
+      const float k = p.rate * softplus_exact(d[e]);
+      const Gates g(ga.get(e), gx.get(e), k, -k * kLog2e);
+      h[e] = __builtin_fmaf(g.a, before.get(e), g.m() * g.i * x.get(e));
+    }
+    st.store(state, h);
+    at.store(out, h);
   }
 }
 
 template <typename T, typename S> int run_step(const GatedStepParams &p, hipStream_t st) {
-  gated_step_kernel<T, S, 1, false><<<dim3((p.dim + 255) / 256, p.batch), 256, 0, st>>>(p);
+  const dim3 grid((p.dim + kThreads * kV - 1) / (kThreads * kV), min(p.batch, 65535));
+  if (p.dim % kV == 0) gated_step_kernel<T, S, true><<<grid, kThreads, 0, st>>>(p);
+  else gated_step_kernel<T, S, false><<<grid, kThreads, 0, st>>>(p);
   return hipGetLastError() == hipSuccess ? MAMBA_OK : MAMBA_E_LAUNCH;
 }
 template <typename T> int step_state(const GatedStepParams &p, hipStream_t st) {
@@ -50,7 +64,6 @@ extern "C" int gated_state_update(const GatedStepParams *p, mamba_stream_t strea
   if (!p->state_batch_indices && p->state_rows < p->batch) return MAMBA_E_BADARG;
   if (p->state_dtype < MAMBA_F32 || p->state_dtype > MAMBA_F16 || p->decay_dtype < MAMBA_F32 || p->decay_dtype > MAMBA_F16)
     return MAMBA_E_BADARG;
-  if (p->batch > 65535) return MAMBA_E_UNSUPPORTED;
   hipStream_t st = static_cast<hipStream_t>(stream);
   switch (p->dtype) {
     case MAMBA_F32: return step_state<float>(*p, st);

@@ -126,6 +126,8 @@ struct Sums {
   float *next_w, *q, *next_b, *p;
 };
 
+// Rows of more than 12 waves leave a thread 128 registers: the parameters are then read again for every row (from the
+// caches) and the next row is not asked for ahead.
 template <typename T, typename R, bool FULL, bool GATE, bool WHOLE, int MAXT>
 __global__ __launch_bounds__(MAXT) void norm_block_bwd_kernel(const NormBlockParams p, const Sums sums) {
   __shared__ float lds[64];
@@ -150,12 +152,18 @@ __global__ __launch_bounds__(MAXT) void norm_block_bwd_kernel(const NormBlockPar
     seg.fetch(gp + r * p.dout_rs, bg);
     seg.fetch(dp + r * dp_rs, bd);
   };
-  fetch(blockIdx.x);
+  constexpr bool LEAN = MAXT > 768;
   float w1[1][8], w2[1][8], sc[1][8], b1[1][8];
-  seg.param(p.norm_weight, p.weight_dtype, 0.f, w1);
-  seg.param(p.scale, p.weight_dtype, p.scale_value, sc);
-  seg.param(p.next_weight, p.weight_dtype, 0.f, w2);
-  if constexpr (FULL) seg.param(p.norm_bias, p.weight_dtype, 0.f, b1);
+  auto params = [&]() {
+    seg.param(p.norm_weight, p.weight_dtype, 0.f, w1);
+    seg.param(p.scale, p.weight_dtype, p.scale_value, sc);
+    seg.param(p.next_weight, p.weight_dtype, 0.f, w2);
+    if constexpr (FULL) seg.param(p.norm_bias, p.weight_dtype, 0.f, b1);
+  };
+  if (!LEAN) {
+    fetch(blockIdx.x);
+    params();
+  }
   float a_next[8], a_q[8], a_nb[FULL ? 8 : 1], a_p[FULL ? 8 : 1];
 #pragma unroll
   for (int e = 0; e < 8; ++e) {
@@ -164,13 +172,17 @@ __global__ __launch_bounds__(MAXT) void norm_block_bwd_kernel(const NormBlockPar
   }
   for (int64_t r = blockIdx.x; r < p.rows; r += gridDim.x) {
     float n1[8], z[8], n2[8], g[8], d[8];
+    if (LEAN) {
+      fetch(r);
+      params();
+    }
     seg.get(bx, n1);
     seg.get(br, n2);
     seg.get(bg, g);
     seg.get(bd, d);
     if constexpr (GATE) seg.get(bz, z);
     const f32x4 st = bs;
-    fetch(min(r + gridDim.x, (int64_t)p.rows - 1));
+    if (!LEAN) fetch(min(r + gridDim.x, (int64_t)p.rows - 1));
     float c1 = 0.f, c2 = 0.f;
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
@@ -324,9 +336,9 @@ __global__ __launch_bounds__(kThreads) void norm_block_any_bwd_kernel(const Norm
 
 // ------------------------------------------------------------------ the parameters' gradients
 // The sums of the parts in their order, and the gradients from them: blockIdx.y 0 is the next norm, 1 this one.  16
-// channels per workgroup, 64 slices of the parts.
-__global__ __launch_bounds__(256) void norm_block_sums_kernel(const NormBlockParams p, const Sums sums, int nparts) {
-  constexpr int SLICES = 64;
+// channels per workgroup, 256 slices of the parts.
+__global__ __launch_bounds__(1024) void norm_block_sums_kernel(const NormBlockParams p, const Sums sums, int nparts) {
+  constexpr int SLICES = 256;
   __shared__ f32x4 lds[SLICES][4];
   const int q = threadIdx.x & 3, sl = threadIdx.x >> 2, c = blockIdx.x * 16 + q * 4, dim = p.dim;
   auto total = [&](const float *src) {  // in the threads of slice 0
@@ -387,11 +399,12 @@ __global__ __launch_bounds__(256) void norm_block_sums_kernel(const NormBlockPar
 bool in_registers(int dim) { return dim >= 8 && dim <= 8192; }
 // threads that hold a row, 8 channels each, in whole waves
 int row_threads(int dim) { return wide_threads((dim + 7) / 8 * 8); }
-// Workgroups that a launch deals its rows to: what the chip holds at once.
-int resident(int dim, bool bwd) {
-  const int t = row_threads(dim);
-  return cu_count() * wide_resident(t, t > 512 ? 4 : bwd ? 3 : 5);
-}
+// Workgroups that a launch deals its rows to.
+// Forward, three waves a SIMD: 112 us at 16384 x 2560 (five 123, one 109), 12.5 at 4096 x 768 in fp32 (14.5, 18.8).
+int fwd_wgs(int dim) { return cu_count() * wide_resident(row_threads(dim), 3); }
+// Backward, every one more is a row of partial sums to write and read: four waves a CU, one workgroup at least.  (Four times
+// as many: 173 -> 193 us at 16384 x 2560, 27 -> 36 us at 4096 x 768 in fp32.)
+int bwd_wgs(int dim) { return cu_count() * max(1, 4 * 64 / row_threads(dim)); }
 
 int check(const NormBlockParams *p, bool bwd) {
   if (!p || !p->x || !p->residual || !p->norm_weight || !p->next_weight) return MAMBA_E_BADARG;
@@ -411,13 +424,13 @@ int check(const NormBlockParams *p, bool bwd) {
 template <typename T, typename R, bool FULL, bool GATE, bool WHOLE>
 void launch_rows(const NormBlockParams &p, const Sums *sums, int wgs, hipStream_t st) {
   const int t = row_threads(p.dim);
-  if (t <= 512) {
-    if (sums) norm_block_bwd_kernel<T, R, FULL, GATE, WHOLE, 512><<<dim3(wgs), dim3(t), 0, st>>>(p, *sums);
-    else norm_block_fwd_kernel<T, R, FULL, GATE, WHOLE, 512><<<dim3(wgs), dim3(t), 0, st>>>(p);
-  } else {
-    if (sums) norm_block_bwd_kernel<T, R, FULL, GATE, WHOLE, 1024><<<dim3(wgs), dim3(t), 0, st>>>(p, *sums);
-    else norm_block_fwd_kernel<T, R, FULL, GATE, WHOLE, 1024><<<dim3(wgs), dim3(t), 0, st>>>(p);
-  }
+  auto go = [&](auto most) {
+    if (sums) norm_block_bwd_kernel<T, R, FULL, GATE, WHOLE, most.value><<<dim3(wgs), dim3(t), 0, st>>>(p, *sums);
+    else norm_block_fwd_kernel<T, R, FULL, GATE, WHOLE, most.value><<<dim3(wgs), dim3(t), 0, st>>>(p);
+  };
+  if (t <= 512) go(std::integral_constant<int, 512>{});
+  else if (t <= 768) go(std::integral_constant<int, 768>{});
+  else go(std::integral_constant<int, 1024>{});
 }
 
 template <typename T, typename R> int run(const NormBlockParams &p, bool bwd, hipStream_t st) {
@@ -431,7 +444,7 @@ template <typename T, typename R> int run(const NormBlockParams &p, bool bwd, hi
     if (p.norm_bias) sums.p = part();
   }
   if (in_registers(p.dim)) {
-    const int wgs = bwd ? nparts : min(p.rows, resident(p.dim, false));
+    const int wgs = bwd ? nparts : min(p.rows, fwd_wgs(p.dim));
     const Sums *s = bwd ? &sums : nullptr;
     const bool full = !p.is_rms || p.norm_bias || p.next_bias, gate = p.z, whole = p.dim % 8 == 0;
     auto pick = [&](auto f, auto g) {
@@ -447,7 +460,7 @@ template <typename T, typename R> int run(const NormBlockParams &p, bool bwd, hi
   }
   if (hipGetLastError() != hipSuccess) return MAMBA_E_LAUNCH;
   if (!bwd) return MAMBA_OK;
-  norm_block_sums_kernel<<<dim3((p.dim + 15) / 16, 2), dim3(256), 0, st>>>(p, sums, nparts);
+  norm_block_sums_kernel<<<dim3((p.dim + 15) / 16, 2), dim3(1024), 0, st>>>(p, sums, nparts);
   return hipGetLastError() == hipSuccess ? MAMBA_OK : MAMBA_E_LAUNCH;
 }
 
@@ -474,5 +487,5 @@ extern "C" int norm_block_bwd(const NormBlockParams *p, mamba_stream_t stream) {
 }
 extern "C" int norm_block_bwd_nparts(const NormBlockParams *p) {
   if (!p || p->rows <= 0 || p->dim <= 0) return MAMBA_E_BADARG;
-  return min(p->rows, in_registers(p->dim) ? resident(p->dim, true) : 1024);
+  return min(p->rows, in_registers(p->dim) ? bwd_wgs(p->dim) : 1024);
 }
