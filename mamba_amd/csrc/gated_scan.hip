@@ -13,6 +13,9 @@
 
 namespace {
 
+constexpr int kV = 2, kTileChannels = 64 * kV;
+constexpr int kSaved = 32;  // positions from one saved state to the next
+
 // The decay's constants of a lane's channels.
 template <int V> struct Rates {
   Vec<V> d, k, k2;
@@ -27,9 +30,9 @@ template <int V> struct Rates {
 };
 
 template <typename T, int V, bool WHOLE, bool PACKED, int R, int NW>
-__global__ __launch_bounds__(NW * 64) void gated_fwd_kernel(const GatedScanParams p, const Chain q, float *ckpt, int ck_rows, int ck_tiles) {
+__global__ __launch_bounds__(NW * 64, 4) void gated_fwd_kernel(const GatedScanParams p, const Chain q, float *ckpt, int saved) {
   __shared__ WaveSteps<V, NW> steps;
-  __shared__ Vec<V> enter[64];
+  __shared__ Ahead<V, NW> ahead;
   __shared__ int ticket;
   const int cgroups = (p.dim + 64 * V - 1) / (64 * V), nchains = cgroups * p.batch;
   const int chain = blockIdx.x % nchains, b = chain / cgroups;
@@ -38,66 +41,88 @@ __global__ __launch_bounds__(NW * 64) void gated_fwd_kernel(const GatedScanParam
   const int n = take_tile(q, chain, &ticket);
   const int t0 = (n * NW + wave) * R, rows = min(max(L - t0, 0), R);
   Rates<V> rate(p, at.c);
-  const T *xp = static_cast<const T *>(p.x) + b * p.x_bs;
-  const T *ap = static_cast<const T *>(p.gate_a) + b * p.gate_a_bs;
-  const T *gp = static_cast<const T *>(p.gate_x) + b * p.gate_x_bs;
   Raw<T, V> x[R], ga[R], gx[R];
+  at.each_kind([&](auto few) {
+    const int64_t from = min(t0, L - 1);
+    const T *xr = static_cast<const T *>(p.x) + b * p.x_bs + from * p.x_ls;
+    const T *ar = static_cast<const T *>(p.gate_a) + b * p.gate_a_bs + from * p.gate_a_ls;
+    const T *gr = static_cast<const T *>(p.gate_x) + b * p.gate_x_bs + from * p.gate_x_ls;
 #pragma unroll
-  for (int j = 0; j < R; ++j) {
-    const int64_t t = min(t0 + j, L - 1);
-    ga[j] = at.load(ap + t * p.gate_a_ls);
-    gx[j] = at.load(gp + t * p.gate_x_ls);
-    x[j] = at.load(xp + t * p.x_ls);
-  }
-  SeqRows<PACKED ? R : 1> rowsof(PACKED ? p.cu_seqlens : nullptr, PACKED ? p.nseq : -1, t0, L);
+    for (int j = 0; j < R; ++j) {  // past the row the last position again and again
+      ga[j] = at.template load<few.value>(ar);
+      gx[j] = at.template load<few.value>(gr);
+      x[j] = at.template load<few.value>(xr);
+      const bool on = t0 + j + 1 < L;
+      ar += on ? p.gate_a_ls : 0, gr += on ? p.gate_x_ls : 0, xr += on ? p.x_ls : 0;
+    }
+  });
+  SeqRows<PACKED ? R : 1> seqs;
+  if constexpr (PACKED) seqs.find(p.cu_seqlens, p.nseq, t0, L);
   rate.form(p.rate);
   Step<V> pos[R], own = no_step<V>();
 #pragma unroll
   for (int j = 0; j < R; ++j) {
 #pragma unroll
     for (int e = 0; e < V; ++e) {
-      const Gates g(ga[j].get(e), gx[j].get(e), rate.k[e], rate.k2[e]);
+      const Gates g(at.get(ga[j], e), at.get(gx[j], e), rate.k[e], rate.k2[e]);
       pos[j].a[e] = PACKED ? fmaxf(g.a, kTiny) : g.a;
-      pos[j].b[e] = g.m() * g.i * x[j].get(e);
+      pos[j].b[e] = g.m() * g.i * at.get(x[j], e);
     }
-    if constexpr (PACKED) {
-      if (!(rowsof.in >> j & 1)) {
-        pos[j].a = pos[j].b = vec_of<V>(0.f);
-      } else if (rowsof.start >> j & 1) {
-        if (p.initial_states) pos[j].b = apply<false>(pos[j], at.load_state(p.initial_states + (int64_t)rowsof.seq[j] * p.dim));
-        pos[j].a = vec_of<V>(0.f);
+    if (!PACKED && j >= rows) pos[j] = no_step<V>();
+    own = then<false>(own, pos[j]);
+  }
+  // a wave with an edge of a sequence among its positions, or with some outside of all: the others never branch
+  const bool edges = PACKED && seqs.edges();
+  if constexpr (PACKED) {
+#pragma unroll
+    for (int e = 0; e < V; ++e) own.a[e] = fmaxf(own.a[e], kTiny);
+    if (edges) {
+      own = no_step<V>();
+#pragma unroll
+      for (int j = 0; j < R; ++j) {
+        if (!(seqs.in >> j & 1)) {
+          pos[j].a = pos[j].b = vec_of<V>(0.f);
+        } else if (seqs.start >> j & 1) {
+          if (p.initial_states) pos[j].b = apply<false>(pos[j], at.load_state(p.initial_states + (int64_t)seqs.seq[j] * p.dim));
+          pos[j].a = vec_of<V>(0.f);
+        }
+        own = then<true>(own, pos[j]);
       }
-    } else {
-      if (j >= rows) pos[j] = no_step<V>();
     }
-    own = then<PACKED>(own, pos[j]);
   }
   steps.put(wave, lane, own);
   lds_barrier();
   Step<V> before = no_step<V>();
   for (int w = 0; w < wave; ++w) before = then<PACKED>(before, steps.get(w, lane));
   if (wave == NW - 1) leave_step(q, chain, n, lane, then<PACKED>(before, own));
-  if (wave == 0) {
-    Vec<V> first = vec_of<V>(0.f);
-    if (!PACKED && p.initial_states) first = at.load_state(p.initial_states + (int64_t)b * p.dim);
-    enter[lane] = entering<PACKED>(q, chain, n, lane, first);
-  }
+  Vec<V> first = vec_of<V>(0.f);
+  if (!PACKED && wave == 0 && p.initial_states) first = at.load_state(p.initial_states + (int64_t)b * p.dim);
+  ahead.template read<PACKED>(q, chain, n, wave, lane, first);
   lds_barrier();
-  Vec<V> h = apply<PACKED>(before, enter[lane]);
+  Vec<V> h = apply<PACKED>(before, ahead.template enter<PACKED>(q, lane));
   if (wave == NW - 1) leave_state(q, chain, n, lane, apply<PACKED>(own, h));
-  if (t0 % ck_rows == 0 && rows > 0) {
-    float *ck = ckpt + (((int64_t)chain * ck_tiles + t0 / ck_rows) * 64 + lane) * V;
+  if (t0 % kSaved == 0 && rows > 0) {
+    float *ck = ckpt + (((int64_t)chain * saved + t0 / kSaved) * 64 + lane) * V;
 #pragma unroll
     for (int e = 0; e < V; ++e) ck[e] = h[e];
   }
-  T *op = static_cast<T *>(p.out) + b * p.out_bs;
+  T *out = static_cast<T *>(p.out) + b * p.out_bs + (int64_t)t0 * p.out_ls;
+  auto write = [&](auto with_edges) {
 #pragma unroll
-  for (int j = 0; j < R; ++j) {
-    h = apply<PACKED>(pos[j], h);
-    if (j < rows) at.store(op + (int64_t)(t0 + j) * p.out_ls, h);
-    if constexpr (PACKED) {
-      if (p.final_states && (rowsof.last >> j & 1)) at.store_state(p.final_states + (int64_t)rowsof.seq[j] * p.dim, h);
+    for (int j = 0; j < R; ++j) {
+      h = apply<with_edges.value>(pos[j], h);
+      if (j < rows) at.store(out, h);
+      out += p.out_ls;
+      if constexpr (with_edges.value) {
+        if (p.final_states && (seqs.last >> j & 1)) at.store_state(p.final_states + (int64_t)seqs.seq[j] * p.dim, h);
+      }
     }
+  };
+  if constexpr (PACKED) {
+    if (edges) write(std::true_type{});
+    else write(std::false_type{});
+  } else {
+    write(std::false_type{});
   }
   if (!PACKED && p.final_states && t0 < L && t0 + R >= L) at.store_state(p.final_states + (int64_t)b * p.dim, h);
   if constexpr (PACKED) {
@@ -111,9 +136,9 @@ __global__ __launch_bounds__(NW * 64) void gated_fwd_kernel(const GatedScanParam
 
 // Tiles from the last one on: what enters a tile is a_t g_t of the position behind it.
 template <typename T, int V, bool WHOLE, bool PACKED, int R, int NW>
-__global__ __launch_bounds__(NW * 64) void gated_bwd_kernel(const GatedScanParams p, const Chain q, const float *ckpt, float *parts) {
+__global__ __launch_bounds__(NW * 64, NW > 4 ? 2 : 3) void gated_bwd_kernel(const GatedScanParams p, const Chain q, const float *ckpt, int saved, float *parts) {
   __shared__ WaveSteps<V, NW> steps, back;
-  __shared__ Vec<V> enter[64];
+  __shared__ Ahead<V, NW> ahead;
   __shared__ int ticket;
   const int cgroups = (p.dim + 64 * V - 1) / (64 * V), nchains = cgroups * p.batch;
   const int chain = blockIdx.x % nchains, b = chain / cgroups;
@@ -123,73 +148,106 @@ __global__ __launch_bounds__(NW * 64) void gated_bwd_kernel(const GatedScanParam
   const int t0 = (tile * NW + wave) * R, rows = min(max(L - t0, 0), R);
   Rates<V> rate(p, at.c);
   Vec<V> h;
-  const float *ck = ckpt + (((int64_t)chain * q.ntiles + tile) * 64 + lane) * V;
+  const float *ck = ckpt + (((int64_t)chain * saved + tile * (R * NW / kSaved)) * 64 + lane) * V;
 #pragma unroll
   for (int e = 0; e < V; ++e) h[e] = ck[e];
-  const T *xp = static_cast<const T *>(p.x) + b * p.x_bs;
-  const T *ap = static_cast<const T *>(p.gate_a) + b * p.gate_a_bs;
-  const T *gp = static_cast<const T *>(p.gate_x) + b * p.gate_x_bs;
-  const T *dp = static_cast<const T *>(p.dout) + b * p.dout_bs;
-  Raw<T, V> x[R], ga[R], gx[R], dout[R];
+  Raw<T, V> x[R], ga[R], gx[R], d[R];
+  at.each_kind([&](auto few) {
+    const int64_t from = min(t0, L - 1);
+    const T *xr = static_cast<const T *>(p.x) + b * p.x_bs + from * p.x_ls;
+    const T *ar = static_cast<const T *>(p.gate_a) + b * p.gate_a_bs + from * p.gate_a_ls;
+    const T *gr = static_cast<const T *>(p.gate_x) + b * p.gate_x_bs + from * p.gate_x_ls;
+    const T *dr = static_cast<const T *>(p.dout) + b * p.dout_bs + from * p.dout_ls;
 #pragma unroll
-  for (int j = 0; j < R; ++j) {
-    const int64_t t = min(t0 + j, L - 1);
-    ga[j] = at.load(ap + t * p.gate_a_ls);
-    gx[j] = at.load(gp + t * p.gate_x_ls);
-    x[j] = at.load(xp + t * p.x_ls);
-    dout[j] = at.load(dp + t * p.dout_ls);
-  }
-  SeqRows<PACKED ? R : 1> rowsof(PACKED ? p.cu_seqlens : nullptr, PACKED ? p.nseq : -1, t0, L);
-  auto starts = [&](int j) { return PACKED && (rowsof.start >> j & 1); };
-  auto ends = [&](int j) { return PACKED && (rowsof.last >> j & 1); };
-  auto counts = [&](int j) { return PACKED ? (rowsof.in >> j & 1) != 0 : j < rows; };
-  auto state_of = [&](int j) { return (int64_t)rowsof.seq[PACKED ? j : 0] * p.dim; };
+    for (int j = 0; j < R; ++j) {
+      ga[j] = at.template load<few.value>(ar);
+      gx[j] = at.template load<few.value>(gr);
+      x[j] = at.template load<few.value>(xr);
+      d[j] = at.template load<few.value>(dr);
+      const bool on = t0 + j + 1 < L;
+      ar += on ? p.gate_a_ls : 0, gr += on ? p.gate_x_ls : 0, xr += on ? p.x_ls : 0, dr += on ? p.dout_ls : 0;
+    }
+  });
+  SeqRows<PACKED ? R : 1> seqs;
+  if constexpr (PACKED) seqs.find(p.cu_seqlens, p.nseq, t0, L);
+  // a wave with an edge of a sequence among its positions, or with some outside of all: the others never branch
+  const bool edges = PACKED && seqs.edges();
+  auto either = [&](auto f) {  // f(whether to look at the edges)
+    if constexpr (PACKED) {
+      if (edges) f(std::true_type{});
+      else f(std::false_type{});
+    } else {
+      f(std::false_type{});
+    }
+  };
+  auto starts = [&](int j) { return (seqs.start >> (PACKED ? j : 0) & 1) != 0; };
+  auto ends = [&](int j) { return (seqs.last >> (PACKED ? j : 0) & 1) != 0; };
+  auto inside = [&](int j) { return (seqs.in >> (PACKED ? j : 0) & 1) != 0; };
+  auto state_of = [&](int j) { return (int64_t)seqs.seq[PACKED ? j : 0] * p.dim; };
   auto initial = [&](int j) { return p.initial_states ? at.load_state(p.initial_states + state_of(j)) : vec_of<V>(0.f); };
+  auto behind_end = [&](int j) { return p.dfinal_states ? at.load_state(p.dfinal_states + state_of(j)) : vec_of<V>(0.f); };
   rate.form(p.rate);
-  // of every position: a, r, i, m, x, the gradient that arrives there, and f: first r / m, then e / g
-  Vec<V> a[R], r[R], i[R], m[R], f[R], xs[R], d[R];
-  Step<V> own = no_step<V>();
+  // of every position, beside x and the gradient that arrives there as they were loaded: a, r, i, m, and f: first r / m,
+  // then e / g
+  Vec<V> a[R], r[R], i[R], m[R], f[R];
 #pragma unroll
   for (int j = 0; j < R; ++j) {
 #pragma unroll
     for (int e = 0; e < V; ++e) {
-      const Gates g(ga[j].get(e), gx[j].get(e), rate.k[e], rate.k2[e]);
+      const Gates g(at.get(ga[j], e), at.get(gx[j], e), rate.k[e], rate.k2[e]);
       const float im = g.im();
       a[j][e] = PACKED ? fmaxf(g.a, kTiny) : g.a;
       r[j][e] = g.r, i[j][e] = g.i, m[j][e] = g.m2 * im, f[j][e] = g.r * im;
-      xs[j][e] = x[j].get(e), d[j][e] = dout[j].get(e);
     }
-    if (!counts(j)) {
-      // a position past the row hands everything on, one outside of the sequences nothing
-      a[j] = vec_of<V>(PACKED ? 0.f : 1.f);
-      r[j] = m[j] = i[j] = f[j] = xs[j] = d[j] = vec_of<V>(0.f);
-    }
-    if (ends(j) && p.dfinal_states) {
-      const Vec<V> v = at.load_state(p.dfinal_states + state_of(j));
-#pragma unroll
-      for (int e = 0; e < V; ++e) d[j][e] += v[e];
-    }
-    Step<V> s;
-    s.a = a[j];
-#pragma unroll
-    for (int e = 0; e < V; ++e) s.b[e] = m[j][e] * i[j][e] * xs[j][e];
-    if (starts(j)) {
-      s.b = apply<false>(s, initial(j));
-      s.a = vec_of<V>(0.f);
-    }
-    own = then<PACKED>(own, s);
-  }
-  Step<V> rev = no_step<V>();
-#pragma unroll
-  for (int j = R - 1; j >= 0; --j) {
-    const bool cut = ends(j), out = PACKED && !counts(j);
-#pragma unroll
-    for (int e = 0; e < V; ++e) {
-      const float g = cut ? d[j][e] : rev.b[e] + d[j][e];
-      rev.a[e] = cut || out ? 0.f : factor1<PACKED>(rev.a[e], a[j][e]);
-      rev.b[e] = out ? 0.f : a[j][e] * g;
+    if (!PACKED && j >= rows) {  // a position past the row hands everything on
+      a[j] = vec_of<V>(1.f);
+      r[j] = i[j] = m[j] = f[j] = vec_of<V>(0.f);
+      x[j].clear(), d[j].clear();
     }
   }
+  Step<V> own, rev;
+  either([&](auto with_edges) {
+    constexpr bool E = with_edges.value;
+    own = rev = no_step<V>();
+#pragma unroll
+    for (int j = 0; j < R; ++j) {
+      if constexpr (E) {
+        if (!inside(j)) {  // nor does one outside of the sequences hand on anything
+          a[j] = r[j] = i[j] = m[j] = f[j] = vec_of<V>(0.f);
+          x[j].clear(), d[j].clear();
+        }
+      }
+      Step<V> s;
+      s.a = a[j];
+#pragma unroll
+      for (int e = 0; e < V; ++e) s.b[e] = m[j][e] * i[j][e] * at.get(x[j], e);
+      if constexpr (E) {
+        if (starts(j)) {
+          s.b = apply<false>(s, initial(j));
+          s.a = vec_of<V>(0.f);
+        }
+      }
+      own = then<E>(own, s);
+    }
+#pragma unroll
+    for (int j = R - 1; j >= 0; --j) {
+      bool cut = false;
+      if constexpr (E) {
+        cut = ends(j) || !inside(j);
+        if (ends(j)) rev.b = behind_end(j);
+        else if (!inside(j)) rev.b = vec_of<V>(0.f);
+      }
+#pragma unroll
+      for (int e = 0; e < V; ++e) {
+        rev.a[e] = cut ? 0.f : factor1<E>(rev.a[e], a[j][e]);
+        rev.b[e] = a[j][e] * (rev.b[e] + at.get(d[j], e));
+      }
+    }
+    if constexpr (PACKED && !E) {
+#pragma unroll
+      for (int e = 0; e < V; ++e) own.a[e] = fmaxf(own.a[e], kTiny), rev.a[e] = fmaxf(rev.a[e], kTiny);
+    }
+  });
   steps.put(wave, lane, own);
   back.put(wave, lane, rev);
   lds_barrier();
@@ -197,50 +255,60 @@ __global__ __launch_bounds__(NW * 64) void gated_bwd_kernel(const GatedScanParam
   for (int w = NW - 1; w > wave; --w) behind = then<PACKED>(behind, back.get(w, lane));
   if (wave == 0) leave_step(q, chain, n, lane, then<PACKED>(behind, rev));
   for (int w = 0; w < wave; ++w) h = apply<PACKED>(steps.get(w, lane), h);
+  either([&](auto with_edges) {
 #pragma unroll
-  for (int j = 0; j < R; ++j) {
-    if (starts(j)) h = initial(j);
-    if (PACKED && !counts(j)) h = vec_of<V>(0.f);
+    for (int j = 0; j < R; ++j) {
+      if constexpr (with_edges.value) {
+        if (starts(j)) h = initial(j);
+        if (!inside(j)) h = vec_of<V>(0.f);
+      }
 #pragma unroll
-    for (int e = 0; e < V; ++e) {
-      const float ix = i[j][e] * xs[j][e];
-      f[j][e] = a[j][e] * __builtin_fmaf(a[j][e] * ix, f[j][e], -r[j][e] * h[e]);
-      h[e] = __builtin_fmaf(a[j][e], h[e], m[j][e] * ix);
+      for (int e = 0; e < V; ++e) {
+        const float ix = i[j][e] * at.get(x[j], e);
+        f[j][e] = a[j][e] * __builtin_fmaf(a[j][e] * ix, f[j][e], -r[j][e] * h[e]);
+        h[e] = __builtin_fmaf(a[j][e], h[e], m[j][e] * ix);
+      }
     }
-  }
-  if (wave == NW - 1) {
-    Vec<V> first = vec_of<V>(0.f);
-    if (!PACKED && p.dfinal_states) first = at.load_state(p.dfinal_states + (int64_t)b * p.dim);
-    enter[lane] = entering<PACKED>(q, chain, n, lane, first);
-  }
+  });
+  Vec<V> first = vec_of<V>(0.f);
+  if (!PACKED && wave == 0 && p.dfinal_states) first = at.load_state(p.dfinal_states + (int64_t)b * p.dim);
+  ahead.template read<PACKED>(q, chain, n, wave, lane, first);
   lds_barrier();
-  Vec<V> carry = apply<PACKED>(behind, enter[lane]), sum = vec_of<V>(0.f);
+  Vec<V> carry = apply<PACKED>(behind, ahead.template enter<PACKED>(q, lane)), sum = vec_of<V>(0.f);
   if (wave == 0) leave_state(q, chain, n, lane, apply<PACKED>(rev, carry));
-  T *dxp = static_cast<T *>(p.dx) + b * p.dx_bs;
-  T *dap = static_cast<T *>(p.dgate_a) + b * p.dgate_a_bs;
-  T *dgp = static_cast<T *>(p.dgate_x) + b * p.dgate_x_bs;
+  const int64_t end = t0 + R - 1;
+  T *dxr = static_cast<T *>(p.dx) + b * p.dx_bs + end * p.dx_ls;
+  T *dar = static_cast<T *>(p.dgate_a) + b * p.dgate_a_bs + end * p.dgate_a_ls;
+  T *dgr = static_cast<T *>(p.dgate_x) + b * p.dgate_x_bs + end * p.dgate_x_ls;
+  either([&](auto with_edges) {
+    constexpr bool E = with_edges.value;
 #pragma unroll
-  for (int j = R - 1; j >= 0; --j) {
-    Vec<V> dx, da, dg;
+    for (int j = R - 1; j >= 0; --j) {
+      if constexpr (E) {
+        if (ends(j)) carry = behind_end(j);
+        else if (!inside(j)) carry = vec_of<V>(0.f);
+      }
+      Vec<V> dx, da, dg;
 #pragma unroll
-    for (int e = 0; e < V; ++e) {
-      float g = ends(j) ? d[j][e] : d[j][e] + carry[e];
-      if (PACKED && !counts(j)) g = 0.f;
-      const float ee = g * f[j][e];
-      dx[e] = g * m[j][e] * i[j][e];
-      da[e] = rate.k[e] * (1.f - r[j][e]) * ee;
-      dg[e] = dx[e] * xs[j][e] * (1.f - i[j][e]);
-      if (counts(j)) sum[e] += ee;
-      carry[e] = a[j][e] * g;
+      for (int e = 0; e < V; ++e) {
+        const float g = at.get(d[j], e) + carry[e], ee = g * f[j][e];
+        dx[e] = g * m[j][e] * i[j][e];
+        da[e] = rate.k[e] * (1.f - r[j][e]) * ee;
+        dg[e] = dx[e] * at.get(x[j], e) * (1.f - i[j][e]);
+        sum[e] += PACKED || j < rows ? ee : 0.f;
+        carry[e] = a[j][e] * g;
+      }
+      if (j < rows) {
+        at.store(dxr, dx);
+        at.store(dar, da);
+        at.store(dgr, dg);
+      }
+      dxr -= p.dx_ls, dar -= p.dgate_a_ls, dgr -= p.dgate_x_ls;
+      if constexpr (E) {
+        if (starts(j) && p.dinitial_states) at.store_state(p.dinitial_states + state_of(j), carry);
+      }
     }
-    if (j < rows) {
-      const int64_t t = t0 + j;
-      at.store(dxp + t * p.dx_ls, dx);
-      at.store(dap + t * p.dgate_a_ls, da);
-      at.store(dgp + t * p.dgate_x_ls, dg);
-    }
-    if (starts(j) && p.dinitial_states) at.store_state(p.dinitial_states + state_of(j), carry);
-  }
+  });
   if (!PACKED && t0 == 0 && p.dinitial_states) at.store_state(p.dinitial_states + (int64_t)b * p.dim, carry);
   if constexpr (PACKED) {
     if (p.dinitial_states && tile == 0)
@@ -265,45 +333,65 @@ __global__ __launch_bounds__(NW * 64) void gated_bwd_kernel(const GatedScanParam
 }
 
 // ------------------------------------------------------------------ host side
-constexpr int kV = 2, kFwdRows = 16, kFwdWaves = 4, kBwdRows = 4, kBwdWaves = 8, kGroup = 8;
-constexpr int kTileChannels = 64 * kV;
+// A pass's tiles of R positions per wave and NW waves, by its size.
+struct Form {
+  int r, nw;
+};
+int64_t chains_of(const GatedScanParams &p) { return (int64_t)p.batch * ((p.dim + kTileChannels - 1) / kTileChannels); }
+int64_t tiles_of(const GatedScanParams &p, int rows) { return chains_of(p) * (((int64_t)p.seqlen + rows - 1) / rows); }
+Form fwd_form(const GatedScanParams &p) {
+  if (p.seqlen <= 32) return {4, 8};
+  return tiles_of(p, 64) <= 512 ? Form{8, 8} : Form{16, 8};
+}
+Form bwd_form(const GatedScanParams &p) {
+  if (p.seqlen <= 32) return {4, 8};
+  return tiles_of(p, 64) <= 2048 ? Form{8, 8} : Form{8, 4};
+}
+// f(R, NW) as compile-time values
+template <typename F> int with_fwd_form(Form o, F f) {
+  if (o.r == 4) return f(std::integral_constant<int, 4>{}, std::integral_constant<int, 8>{});
+  if (o.r == 8) return f(std::integral_constant<int, 8>{}, std::integral_constant<int, 8>{});
+  return f(std::integral_constant<int, 16>{}, std::integral_constant<int, 8>{});
+}
+template <typename F> int with_bwd_form(Form o, F f) {
+  if (o.r == 4) return f(std::integral_constant<int, 4>{}, std::integral_constant<int, 8>{});
+  if (o.nw == 8) return f(std::integral_constant<int, 8>{}, std::integral_constant<int, 8>{});
+  return f(std::integral_constant<int, 8>{}, std::integral_constant<int, 4>{});
+}
 
 // Tiles of one pass and what its chains need in memory: the tickets and words, cleared before the launch, lie at the
-// start of the buffer, `tail` behind them.
+// start of the buffer, what else it holds behind them.
 struct Plan {
-  int cgroups, ntiles, group, ngroups;
-  int64_t chains, words, head;  // head: bytes before the tail
-  Plan(const GatedScanParams &p, int tile_rows) {
-    cgroups = (p.dim + kTileChannels - 1) / kTileChannels;
-    chains = (int64_t)p.batch * cgroups;
-    ntiles = (int)(((int64_t)p.seqlen + tile_rows - 1) / tile_rows);
-    group = group_of(chains, ntiles);
+  int ntiles, group, ngroups;
+  int64_t chains, steps, head;  // words of steps, bytes of tickets and words
+  Plan(const GatedScanParams &p, Form o) {
+    chains = chains_of(p);
+    ntiles = (int)(tiles_of(p, o.r * o.nw) / chains);
+    group = min(ntiles, chains >= 128 ? 1 : 16);
     ngroups = (ntiles + group - 1) / group;
-    words = ntiles > 1 ? chains * (ntiles + ngroups) * kTileChannels : 0;
-    head = ntiles > 1 ? (chains * 4 + 15) / 16 * 16 + words * 8 : 0;
-  }
-  static int group_of(int64_t chains, int ntiles) {
-    (void)chains;
-    return min(ntiles, kGroup);
+    steps = group > 1 ? chains * ntiles * kTileChannels : 0;  // a group of one tile leaves its state alone
+    head = ntiles > 1 ? (chains * 4 + 15) / 16 * 16 + (steps + chains * ngroups * kTileChannels) * 8 : 0;
   }
   Chain chain(void *buf) const {
     Chain q;
     q.tickets = static_cast<uint32_t *>(buf);
     q.steps = reinterpret_cast<uint64_t *>(static_cast<char *>(buf) + (chains * 4 + 15) / 16 * 16);
-    q.states = q.steps + chains * ntiles * kTileChannels;
+    q.states = q.steps + steps;
     q.ntiles = ntiles, q.group = group, q.ngroups = ngroups;
     return q;
   }
-  bool fits() const { return chains * ntiles <= 0x7fffffff; }
 };
-Plan fwd_plan(const GatedScanParams &p) { return Plan(p, kFwdRows * kFwdWaves); }
-Plan bwd_plan(const GatedScanParams &p) { return Plan(p, kBwdRows * kBwdWaves); }
+int saved_states(const GatedScanParams &p) { return (p.seqlen + kSaved - 1) / kSaved; }
 
 bool shapes_ok(const GatedScanParams *p) {
   if (!p || p->batch <= 0 || p->seqlen <= 0 || p->dim <= 0 || p->nseq < 0) return false;
   if (p->nseq > 0 && p->batch != 1) return false;
   if (!(p->rate >= 0.f && p->rate <= 3.4e38f)) return false;
   return p->dtype >= MAMBA_F32 && p->dtype <= MAMBA_F16 && p->decay_dtype >= MAMBA_F32 && p->decay_dtype <= MAMBA_F16;
+}
+// positions, tiles and workgroups are counted in 32 bits
+bool counts_fit(const GatedScanParams &p) {
+  return p.seqlen <= 0x7fffffff - 4096 && p.nseq <= 0x7fffffff - 64 && p.dim <= 0x7fffffff / 8 && tiles_of(p, 32) <= 0x7fffffff;
 }
 int check(const GatedScanParams *p, bool bwd) {
   if (!shapes_ok(p)) return MAMBA_E_BADARG;
@@ -313,17 +401,15 @@ int check(const GatedScanParams *p, bool bwd) {
   if (!bwd && !p->out) return MAMBA_E_BADARG;
   if (bwd && (!p->dout || !p->dx || !p->dgate_a || !p->dgate_x || !p->ddecay || !p->ws || !aligned16(p->ws)))
     return MAMBA_E_BADARG;
-  // positions and tiles are counted in 32 bits
-  if (p->seqlen > 0x7fffffff - 4096 || p->nseq > 0x7fffffff - 64 || !fwd_plan(*p).fits() || !bwd_plan(*p).fits()) return MAMBA_E_UNSUPPORTED;
-  return MAMBA_OK;
+  return counts_fit(*p) ? MAMBA_OK : MAMBA_E_UNSUPPORTED;
 }
 
-// f(T{}, even, packed) with the call's types as compile-time values
-template <typename F> int with_forms(const GatedScanParams &p, F f) {
+// f(T{}, whole, packed) with the call's types as compile-time values
+template <typename F> int with_types(const GatedScanParams &p, F f) {
   auto forms = [&](auto t) {
-    const bool even = p.dim % kV == 0;
-    if (p.nseq > 0) return even ? f(t, std::true_type{}, std::true_type{}) : f(t, std::false_type{}, std::true_type{});
-    return even ? f(t, std::true_type{}, std::false_type{}) : f(t, std::false_type{}, std::false_type{});
+    const bool whole = p.dim % kV == 0;
+    if (p.nseq > 0) return whole ? f(t, std::true_type{}, std::true_type{}) : f(t, std::false_type{}, std::true_type{});
+    return whole ? f(t, std::true_type{}, std::false_type{}) : f(t, std::false_type{}, std::false_type{});
   };
   switch (p.dtype) {
     case MAMBA_F32: return forms(float{});
@@ -336,40 +422,48 @@ template <typename F> int with_forms(const GatedScanParams &p, F f) {
 
 extern "C" int64_t gated_scan_ckpt_bytes(const GatedScanParams *p) {
   if (!shapes_ok(p)) return MAMBA_E_BADARG;
-  const Plan f = fwd_plan(*p), w = bwd_plan(*p);
-  return f.head + w.chains * w.ntiles * kTileChannels * 4;
+  if (!counts_fit(*p)) return MAMBA_E_UNSUPPORTED;
+  const Plan f(*p, fwd_form(*p));
+  return f.head + f.chains * saved_states(*p) * kTileChannels * 4;
 }
 extern "C" int64_t gated_scan_bwd_ws_bytes(const GatedScanParams *p) {
   if (!shapes_ok(p)) return MAMBA_E_BADARG;
-  const Plan w = bwd_plan(*p);
+  if (!counts_fit(*p)) return MAMBA_E_UNSUPPORTED;
+  const Plan w(*p, bwd_form(*p));
   return w.head + (int64_t)p->batch * w.ntiles * p->dim * 4;
 }
 
 extern "C" int gated_scan_fwd(const GatedScanParams *p, mamba_stream_t stream) {
   if (const int rc = check(p, false)) return rc;
-  const Plan plan = fwd_plan(*p);
+  const Form o = fwd_form(*p);
+  const Plan plan(*p, o);
   if (plan.head > 0)
     if (const int rc = mamba_hip_zero(p->ckpt, plan.head, stream)) return rc;
-  float *ck = reinterpret_cast<float *>(static_cast<char *>(p->ckpt) + plan.head);
-  return with_forms(*p, [&](auto t, auto even, auto packed) {
-    gated_fwd_kernel<decltype(t), kV, even.value, packed.value, kFwdRows, kFwdWaves>
-        <<<dim3((unsigned)(plan.chains * plan.ntiles)), dim3(kFwdWaves * 64), 0, static_cast<hipStream_t>(stream)>>>(
-            *p, plan.chain(p->ckpt), ck, kBwdRows * kBwdWaves, bwd_plan(*p).ntiles);
-    return hipGetLastError() == hipSuccess ? MAMBA_OK : MAMBA_E_LAUNCH;
+  float *saved = reinterpret_cast<float *>(static_cast<char *>(p->ckpt) + plan.head);
+  return with_types(*p, [&](auto t, auto whole, auto packed) {
+    return with_fwd_form(o, [&](auto r, auto nw) {
+      gated_fwd_kernel<decltype(t), kV, whole.value, packed.value, r.value, nw.value>
+          <<<dim3((unsigned)(plan.chains * plan.ntiles)), dim3(nw.value * 64), 0, static_cast<hipStream_t>(stream)>>>(
+              *p, plan.chain(p->ckpt), saved, saved_states(*p));
+      return hipGetLastError() == hipSuccess ? MAMBA_OK : MAMBA_E_LAUNCH;
+    });
   });
 }
 extern "C" int gated_scan_bwd(const GatedScanParams *p, mamba_stream_t stream) {
   if (const int rc = check(p, true)) return rc;
-  const Plan plan = bwd_plan(*p);
+  const Form o = bwd_form(*p);
+  const Plan plan(*p, o);
   if (plan.head > 0)
     if (const int rc = mamba_hip_zero(p->ws, plan.head, stream)) return rc;
   hipStream_t st = static_cast<hipStream_t>(stream);
-  const float *ck = reinterpret_cast<const float *>(static_cast<const char *>(p->ckpt) + fwd_plan(*p).head);
+  const float *saved = reinterpret_cast<const float *>(static_cast<const char *>(p->ckpt) + Plan(*p, fwd_form(*p)).head);
   float *parts = reinterpret_cast<float *>(static_cast<char *>(p->ws) + plan.head);
-  const int rc = with_forms(*p, [&](auto t, auto even, auto packed) {
-    gated_bwd_kernel<decltype(t), kV, even.value, packed.value, kBwdRows, kBwdWaves>
-        <<<dim3((unsigned)(plan.chains * plan.ntiles)), dim3(kBwdWaves * 64), 0, st>>>(*p, plan.chain(p->ws), ck, parts);
-    return hipGetLastError() == hipSuccess ? MAMBA_OK : MAMBA_E_LAUNCH;
+  const int rc = with_types(*p, [&](auto t, auto whole, auto packed) {
+    return with_bwd_form(o, [&](auto r, auto nw) {
+      gated_bwd_kernel<decltype(t), kV, whole.value, packed.value, r.value, nw.value>
+          <<<dim3((unsigned)(plan.chains * plan.ntiles)), dim3(nw.value * 64), 0, st>>>(*p, plan.chain(p->ws), saved, saved_states(*p), parts);
+      return hipGetLastError() == hipSuccess ? MAMBA_OK : MAMBA_E_LAUNCH;
+    });
   });
   if (rc != MAMBA_OK) return rc;
   ReduceJobs jobs{};

@@ -3,8 +3,6 @@
 // loads in flight together; many short waves fill the memory's channels.
 #include "gated_tile.hpp"
 
-#include <type_traits>
-
 namespace {
 
 constexpr int kV = 4, kThreads = 256;
@@ -22,18 +20,22 @@ template <typename T, typename S, bool WHOLE> __global__ __launch_bounds__(kThre
       continue;
     }
     S *state = static_cast<S *>(p.state) + row * p.state_rs;
-    const Raw<T, kV> ga = at.load(static_cast<const T *>(p.gate_a) + b * p.gate_a_rs);
-    const Raw<T, kV> gx = at.load(static_cast<const T *>(p.gate_x) + b * p.gate_x_rs);
-    const Raw<T, kV> x = at.load(static_cast<const T *>(p.x) + b * p.x_rs);
-    const Raw<S, kV> before = st.load(state);
+    Raw<T, kV> ga, gx, x;
+    Raw<S, kV> before;
+    at.each_kind([&](auto few) {
+      ga = at.template load<few.value>(static_cast<const T *>(p.gate_a) + b * p.gate_a_rs);
+      gx = at.template load<few.value>(static_cast<const T *>(p.gate_x) + b * p.gate_x_rs);
+      x = at.template load<few.value>(static_cast<const T *>(p.x) + b * p.x_rs);
+      before = st.template load<few.value>(state);
+    });
     Vec<kV> d, h;
 #pragma unroll
     for (int e = 0; e < kV; ++e) d[e] = ld_param(p.decay, p.decay_dtype, min(c + e, p.dim - 1));
 #pragma unroll
     for (int e = 0; e < kV; ++e) {
       const float k = p.rate * softplus_exact(d[e]);
-      const Gates g(ga.get(e), gx.get(e), k, -k * kLog2e);
-      h[e] = __builtin_fmaf(g.a, before.get(e), g.m() * g.i * x.get(e));
+      const Gates g(at.get(ga, e), at.get(gx, e), k, -k * kLog2e);
+      h[e] = __builtin_fmaf(g.a, st.get(before, e), g.m() * g.i * at.get(x, e));
     }
     st.store(state, h);
     at.store(out, h);

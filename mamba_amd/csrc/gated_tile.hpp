@@ -8,6 +8,8 @@
 #pragma once
 #include "gated_gates.hpp"
 
+#include <type_traits>
+
 namespace {
 
 template <int V> struct Vec {
@@ -33,35 +35,42 @@ template <int W> struct Words<W, 4> {
 
 // V neighbouring channels of one position as they lie in memory.
 template <typename T, int V> struct Raw {
-  static constexpr int W = V * (DT<T>::id == MAMBA_F32 ? 4 : 2) / 4;
+  static constexpr bool HALF = DT<T>::id != MAMBA_F32;
+  static constexpr int W = HALF ? V / 2 : V;
   uint32_t w[W];
+  DEVI void clear() {
+#pragma unroll
+    for (int i = 0; i < W; ++i) w[i] = 0;
+  }
   DEVI float get(int e) const {
-    if constexpr (DT<T>::id == MAMBA_F32) return __builtin_bit_cast(float, w[e]);
+    if constexpr (!HALF) return __builtin_bit_cast(float, w[e]);
     else if constexpr (DT<T>::id == MAMBA_BF16) return e & 1 ? bf16_hi(w[e / 2]) : bf16_lo(w[e / 2]);
     else return e & 1 ? f16_hi(w[e / 2]) : f16_lo(w[e / 2]);
   }
 };
 
-// How a lane reads and writes its channels c .. c + V - 1.  WHOLE: the number of channels is a multiple of V, all of a
-// lane's channels are there or none.  Otherwise a lane at the end reads the last V channels and moves its own to the
-// front.  Rows lie at any alignment (gfx950 serves these accesses at element alignment).  Lanes past the last channel
-// read the last ones again and write nothing.
+// How a lane reads and writes its channels c .. c + V - 1, in one piece at any alignment (gfx950 serves that; rows of 16-bit
+// channels that begin off a word cost a quarter more).  WHOLE: the number of channels is a multiple of V, all of a lane's
+// channels are there or none.  Otherwise a lane at the end reads the row's last V channels, and `get` moves its own to the
+// front; rows of less than V channels (`few`) are read channel by channel.  Lanes past the last channel read the last ones
+// again and write nothing.
 template <typename T, int V, bool WHOLE> struct Lane {
-  static constexpr int W = Raw<T, V>::W;
-  int c, n;         // the lane's first channel, how many of its channels are there
-  int dim, shift;   // the channel read first lies `shift` before c
-  uint32_t at, to;  // byte offsets in a row: of what is read, of c
-  DEVI Lane(int c_, int dim_) : c(c_), dim(dim_) {
+  typedef Raw<T, V> R;
+  int c, n, dim;     // the lane's first channel, how many of its channels are there, those of a row
+  int shift;         // how far before c the channel read first lies
+  uint32_t at, to;   // byte offsets in a row: of what is read, of c
+  bool few;
+  DEVI Lane(int c_, int dim_) : c(c_), dim(dim_), few(!WHOLE && dim_ < V) {
     n = min(max(dim - c, 0), V);
     const int from = max(min(c, dim - V), 0);
-    shift = min(c - from, V - 1);
+    shift = WHOLE ? 0 : min(c - from, V - 1);
     at = (uint32_t)from * sizeof(T);
     to = (uint32_t)c * sizeof(T);
   }
-  DEVI Raw<T, V> load(const T *row) const {
-    Raw<T, V> r;
+  template <bool FEW = false> DEVI R load(const T *row) const {
+    R r;
     const GLOBAL_AS char *p = (const GLOBAL_AS char *)row;
-    if (!WHOLE && dim < V) {  // fewer channels in a row than a lane holds
+    if constexpr (FEW) {
       uint32_t q[V];
 #pragma unroll
       for (int e = 0; e < V; ++e) {
@@ -70,47 +79,50 @@ template <typename T, int V, bool WHOLE> struct Lane {
         else q[e] = *(const GLOBAL_AS uint16_t *)(p + o);
       }
 #pragma unroll
-      for (int e = 0; e < V; ++e) {
-        if constexpr (sizeof(T) == 4) r.w[e] = q[e];
-        else if (e & 1) r.w[e / 2] = q[e - 1] | q[e] << 16;
-      }
-      return r;
-    }
-    typedef typename Words<W, sizeof(T)>::type words;
-    const words v = *(const GLOBAL_AS words *)(p + at);
+      for (int i = 0; i < R::W; ++i) r.w[i] = R::HALF ? q[2 * i] | q[2 * i + 1] << 16 : q[i];
+    } else {
+      typedef typename Words<R::W, sizeof(T)>::type words;
+      const words v = *(const GLOBAL_AS words *)(p + at);
 #pragma unroll
-    for (int i = 0; i < W; ++i) r.w[i] = v[i];
-    if constexpr (!WHOLE) {
-#pragma unroll
-      for (int step = V / 2; step >= 1; step >>= 1) {  // move by `step` channels where shift says so
-        const bool on = shift & step;
-#pragma unroll
-        for (int i = 0; i < W; ++i) {
-          uint32_t up;
-          if constexpr (sizeof(T) == 4) up = i + step < W ? r.w[i + step] : 0u;
-          else if (step >= 2) up = i + step / 2 < W ? r.w[i + step / 2] : 0u;
-          else up = r.w[i] >> 16 | (i + 1 < W ? r.w[i + 1] << 16 : 0u);
-          r.w[i] = on ? up : r.w[i];
-        }
-      }
+      for (int i = 0; i < R::W; ++i) r.w[i] = v[i];
     }
     return r;
   }
-  DEVI void store(T *row, const Vec<V> &x) const {
-    typedef typename Words<W, sizeof(T)>::type words;
-    GLOBAL_AS char *p = (GLOBAL_AS char *)row + to;
-    if (n == V) {
-      words v;
+  DEVI float get(const R &r, int e) const {
+    if constexpr (WHOLE) {
+      return r.get(e);
+    } else {
+      float v = r.get(e);
 #pragma unroll
-      for (int i = 0; i < W; ++i) {
-        if constexpr (DT<T>::id == MAMBA_F32) v[i] = __builtin_bit_cast(uint32_t, x.v[i]);
-        else if constexpr (DT<T>::id == MAMBA_BF16) v[i] = pack_bf16(x.v[2 * i], x.v[2 * i + 1]);
-        else v[i] = pack_f16(x.v[2 * i], x.v[2 * i + 1]);
-      }
-      *(GLOBAL_AS words *)p = v;
+      for (int s = 1; s < V; ++s)
+        if (e + s < V) v = shift == s ? r.get(e + s) : v;
+      return v;
+    }
+  }
+  // of rows of less than V channels and of others: f(rows of few channels), so that one branch stands around all loads
+  template <typename F> DEVI void each_kind(F f) const {
+    if constexpr (WHOLE) {
+      f(std::false_type{});
+    } else {
+      if (few) f(std::true_type{});
+      else f(std::false_type{});
+    }
+  }
+  DEVI void store(T *row, const Vec<V> &x) const {
+    typedef typename Words<R::W, sizeof(T)>::type words;
+    GLOBAL_AS char *p = (GLOBAL_AS char *)row;
+    words v;
+#pragma unroll
+    for (int i = 0; i < R::W; ++i) {
+      if constexpr (DT<T>::id == MAMBA_F32) v[i] = __builtin_bit_cast(uint32_t, x.v[i]);
+      else if constexpr (DT<T>::id == MAMBA_BF16) v[i] = pack_bf16(x.v[2 * i], x.v[2 * i + 1]);
+      else v[i] = pack_f16(x.v[2 * i], x.v[2 * i + 1]);
+    }
+    if (n == V) {
+      *(GLOBAL_AS words *)(p + to) = v;
     } else if (!WHOLE) {
 #pragma unroll
-      for (int e = 0; e < V; ++e)
+      for (int e = 0; e < V - 1; ++e)
         if (e < n) st1<T>(row + c + e, x[e]);
     }
   }
@@ -188,7 +200,7 @@ template <int V, int NW> struct WaveSteps {
 // are started.
 struct Chain {
   uint32_t *tickets;  // one per chain (row and channel group)
-  uint64_t *steps;    // (chain, ntiles, 64 V)
+  uint64_t *steps;    // (chain, ntiles, 64 V), none where a group is one tile
   uint64_t *states;   // (chain, ngroups, 64 V)
   int ntiles, group, ngroups;
 };
@@ -204,14 +216,21 @@ template <int V> DEVI void put_words(uint64_t *p, const Step<V> &s) {
   for (int e = 0; e < V; ++e) __hip_atomic_store(p + e, word_of(s.a[e], s.b[e]), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
 
-// Whole wave: the words of every lane for N tiles, 64 V words apart, once all of them are there.
-template <int V, int N> DEVI void wait_words(const uint64_t *p, uint64_t (&w)[N][V]) {
+// Whole wave: the words of every lane for the tiles from p on, 64 V words apart, once those of the first `count` are there
+// (at least one; the others repeat the last).
+template <int V, int N> DEVI void wait_words(const uint64_t *p, int count, uint64_t (&w)[N][V]) {
+  // Until they are there the first words of the tiles alone are asked for, a tile by each lane: whole words asked for again and
+  // again by every waiting wave take the memory's paths from the tiles that still load (34 -> 45 us at 2 x 2048 x 1536).
+  const int lane = threadIdx.x & 63;
+  const uint64_t *hint = p - lane * V + (int64_t)min(lane, count - 1) * 64 * V;
+  while (!__all((__hip_atomic_load(hint, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) & kThere) != 0)) __builtin_amdgcn_s_sleep(4);
   for (;;) {
     uint64_t all = kThere;
 #pragma unroll
     for (int i = 0; i < N; ++i)
 #pragma unroll
-      for (int e = 0; e < V; ++e) w[i][e] = __hip_atomic_load(p + i * 64 * V + e, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      for (int e = 0; e < V; ++e)
+        w[i][e] = __hip_atomic_load(p + min(i, count - 1) * 64 * V + e, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 #pragma unroll
     for (int i = 0; i < N; ++i)
 #pragma unroll
@@ -221,38 +240,51 @@ template <int V, int N> DEVI void wait_words(const uint64_t *p, uint64_t (&w)[N]
   }
 }
 
-// Whole wave: the state that enters tile n of the chain; `first` is the one that enters tile 0.
-template <bool RESETS, int V> DEVI Vec<V> entering(const Chain &q, int64_t chain, int n, int lane, Vec<V> first) {
-  const int g = n / q.group, from = g * q.group, count = n - from;
-  const uint64_t *sp = q.steps + (chain * q.ntiles + from) * (64 * V) + lane * V;
-  Step<V> s = no_step<V>();
-  auto take = [&](const uint64_t (&w)[V]) {
-    Step<V> next;
+// What lies before tile n in its chain, read by all waves of the workgroup at once: wave w composes the w-th part of the
+// steps before it in its group, wave 0 reads the state at the end of the group before (`first` enters tile 0).  After the
+// next barrier `enter` has the state that enters tile n.
+template <int V, int NW> struct Ahead {
+  WaveSteps<V, NW> steps;
+  Vec<V> state[64];
+  template <bool RESETS> DEVI void read(const Chain &q, int64_t chain, int n, int wave, int lane, Vec<V> first) {
+    constexpr int N = 4;
+    const int g = n / q.group, from = g * q.group, count = n - from, part = (count + NW - 1) / NW;
+    const int lo = min(wave * part, count), hi = min(lo + part, count);
+    const uint64_t *sp = q.steps + (chain * q.ntiles + from) * (64 * V) + lane * V;
+    Step<V> s = no_step<V>();
+    for (int i = lo; i < hi; i += N) {
+      uint64_t w[N][V];
+      wait_words<V, N>(sp + (int64_t)i * 64 * V, min(N, hi - i), w);
 #pragma unroll
-    for (int e = 0; e < V; ++e) next.a[e] = word_a(w[e]), next.b[e] = word_b(w[e]);
-    s = then<RESETS>(s, next);
-  };
-  int i = 0;
-  constexpr int B = 4;
-  for (; i + B <= count; i += B) {
-    uint64_t w[B][V];
-    wait_words<V, B>(sp + (int64_t)i * 64 * V, w);
+      for (int j = 0; j < N; ++j) {
+        if (i + j < hi) {
+          Step<V> next;
 #pragma unroll
-    for (int j = 0; j < B; ++j) take(w[j]);
-  }
-  for (; i < count; ++i) {
-    uint64_t w[1][V];
-    wait_words<V, 1>(sp + (int64_t)i * 64 * V, w);
-    take(w[0]);
-  }
-  if (g > 0) {
-    uint64_t w[1][V];
-    wait_words<V, 1>(q.states + (chain * q.ngroups + g - 1) * (64 * V) + lane * V, w);
+          for (int e = 0; e < V; ++e) next.a[e] = word_a(w[j][e]), next.b[e] = word_b(w[j][e]);
+          s = then<RESETS>(s, next);
+        }
+      }
+    }
+    steps.put(wave, lane, s);
+    if (wave == 0) {
+      if (g > 0) {
+        uint64_t w[1][V];
+        wait_words<V, 1>(q.states + (chain * q.ngroups + g - 1) * (64 * V) + lane * V, 1, w);
 #pragma unroll
-    for (int e = 0; e < V; ++e) first[e] = word_b(w[0][e]);
+        for (int e = 0; e < V; ++e) first[e] = word_b(w[0][e]);
+      }
+      state[lane] = first;
+    }
   }
-  return apply<RESETS>(s, first);
-}
+  template <bool RESETS> DEVI Vec<V> enter(const Chain &q, int lane) const {
+    Vec<V> h = state[lane];
+    if (q.group > 1) {
+#pragma unroll
+      for (int w = 0; w < NW; ++w) h = apply<RESETS>(steps.get(w, lane), h);
+    }
+    return h;
+  }
+};
 // What tile n leaves for the ones behind it: its step at once, the state at its end where it closes a group.
 template <int V> DEVI void leave_step(const Chain &q, int64_t chain, int n, int lane, const Step<V> &s) {
   if (n + 1 < q.ntiles && (n + 1) % q.group != 0) put_words<V>(q.steps + (chain * q.ntiles + n) * (64 * V) + lane * V, s);
@@ -278,9 +310,11 @@ DEVI int bound_at(const int32_t *cu, int s, int L) {
   return min(max(v, 0), L);
 }
 template <int R> struct SeqRows {
-  uint32_t start = 0, last = 0, in = 0;
+  uint32_t start, last, in;
   int seq[R];
-  DEVI SeqRows(const int32_t *cu, int nseq, int t0, int L) {
+  DEVI bool edges() const { return (start | last) != 0 || in != (1u << R) - 1; }
+  DEVI void find(const int32_t *cu, int nseq, int t0, int L) {
+    start = last = in = 0;
     int lo = -1, hi = nseq + 1;  // the last bound at or before t0
     while (hi - lo > 1) {
       const int mid = (lo + hi) >> 1;

@@ -32,15 +32,17 @@ def gated_linear_oracle(x, gate_a, gate_x, decay, rate=8.0, initial_states=None,
     ddecay, dinitial.  cu_seqlens: a list."""
     x, ga, gx, lam = _d(x), _d(gate_a), _d(gate_x), _d(decay)
     batch, L, dim = x.shape
+    # sequences as (their states, their row, first position, end); the rows of a batch are walked together
     if cu_seqlens is None:
-        spans = [(b, 0, L) for b in range(batch)]
+        spans = [(slice(None), slice(None), 0, L)]
     else:
-        spans = [(0, cu_seqlens[q], cu_seqlens[q + 1]) for q in range(len(cu_seqlens) - 1)]
+        spans = [(q, 0, cu_seqlens[q], cu_seqlens[q + 1]) for q in range(len(cu_seqlens) - 1)]
+    seqs = batch if cu_seqlens is None else len(spans)
     inside = torch.zeros(batch, L, 1, dtype=torch.float64)
-    for row, lo, hi in spans:
+    for _, row, lo, hi in spans:
         inside[row, lo:hi] = 1
     x, ga, gx = (torch.where(inside > 0, t, torch.zeros_like(t)) for t in (x, ga, gx))
-    init = _d(initial_states) if initial_states is not None else torch.zeros(len(spans), dim, dtype=torch.float64)
+    init = _d(initial_states) if initial_states is not None else torch.zeros(seqs, dim, dtype=torch.float64)
     r, i = torch.sigmoid(ga), torch.sigmoid(gx)
     k = rate * torch.nn.functional.softplus(lam, threshold=1e9)
     a = torch.exp(-k * r)
@@ -48,14 +50,15 @@ def gated_linear_oracle(x, gate_a, gate_x, decay, rate=8.0, initial_states=None,
     b = m * i * x
     Ca = C + k * r * (8 + 2 * ga.abs().clamp(max=100.0))
     tiny = 2.0 ** -62 * k.clamp(min=1.0).sqrt()
+    small, size_b = tiny * (i * x).abs(), b.abs()
     h, before = torch.zeros_like(x), torch.zeros_like(x)
     Eh, Ebefore, final, Efinal = torch.zeros_like(x), torch.zeros_like(x), init.clone(), torch.zeros_like(init)
-    for q, (row, lo, hi) in enumerate(spans):
-        now, H, E = init[q].clone(), init[q].abs(), torch.zeros(dim, dtype=torch.float64)
+    for q, row, lo, hi in spans:
+        now, H, E = init[q].clone(), init[q].abs(), torch.zeros_like(init[q])
         for t in range(lo, hi):
             before[row, t], Ebefore[row, t] = now, E
-            E = a[row, t] * E + U * Ca[row, t] * (a[row, t] * H + 2 * b[row, t].abs()) + tiny * (i * x)[row, t].abs()
-            H = a[row, t] * H + b[row, t].abs()
+            E = a[row, t] * E + U * Ca[row, t] * (a[row, t] * H + 2 * size_b[row, t]) + small[row, t]
+            H = a[row, t] * H + size_b[row, t]
             now = a[row, t] * now + b[row, t]
             h[row, t], Eh[row, t] = now, E
         final[q], Efinal[q] = now, E
@@ -67,8 +70,8 @@ def gated_linear_oracle(x, gate_a, gate_x, decay, rate=8.0, initial_states=None,
     dout = torch.where(inside > 0, dout, torch.zeros_like(dout))
     g, Eg = torch.zeros_like(x), torch.zeros_like(x)
     dinit, Edinit = torch.zeros_like(init), torch.zeros_like(init)
-    for q, (row, lo, hi) in enumerate(spans):
-        carry, H, E = dfinal[q].clone(), dfinal[q].abs(), torch.zeros(dim, dtype=torch.float64)
+    for q, row, lo, hi in spans:
+        carry, H, E = dfinal[q].clone(), dfinal[q].abs(), torch.zeros_like(init[q])
         for t in range(hi - 1, lo - 1, -1):
             g[row, t], Eg[row, t] = dout[row, t] + carry, E + U * (dout[row, t].abs() + H)
             H = a[row, t] * (dout[row, t].abs() + H)

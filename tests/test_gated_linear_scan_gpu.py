@@ -67,6 +67,23 @@ def test_shapes(batch, L, dim, dtype):
     _check(_inputs(batch, L, dim, dtype, seed=L + dim, states=(L + dim) % 3 != 0))
 
 
+# both sides of the lines at which a pass takes other tiles, and rows enough that every tile hands its state on by itself
+@pytest.mark.parametrize("batch,L,dim,dtype", [
+    (2, 32, 130, torch.bfloat16), (2, 33, 130, torch.bfloat16),
+    (16, 64 * 32, 2, torch.float32), (16, 64 * 32 + 1, 2, torch.float32), (9, 3700, 129, torch.bfloat16),
+    (64, 64 * 32, 1, torch.float32), (64, 64 * 32 + 5, 2, torch.bfloat16), (22, 6200, 130, torch.float16),
+    (130, 300, 5, torch.float32), (140, 1000, 2, torch.bfloat16)])
+def test_sizes_of_other_tiles(batch, L, dim, dtype):
+    _check(_inputs(batch, L, dim, dtype, seed=L, states=L % 2 == 0, long_memory=dtype == torch.float32))
+
+
+@pytest.mark.parametrize("total,dim", [(17000, 257), (66100, 129)])
+def test_long_packed_rows(total, dim):
+    g = torch.Generator().manual_seed(total)
+    cu = [0, 3] + (torch.randperm(total - 500, generator=g)[:21] + 20).sort().values.tolist()
+    _check(_inputs(1, total, dim, torch.bfloat16, seqs=len(cu) - 1), cu)
+
+
 @pytest.mark.parametrize("L", [300, 3000])
 def test_long_memory(L):
     """Decays as such layers are initialised: a state lasts for hundreds of positions."""
