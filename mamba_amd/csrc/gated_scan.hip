@@ -29,7 +29,7 @@ template <int V> struct Rates {
   }
 };
 
-template <typename T, int V, bool WHOLE, bool PACKED, int R, int NW>
+template <typename T, int V, bool WHOLE, bool PACKED, int R, int NW, int STREAM>
 __global__ __launch_bounds__(NW * 64, 4) void gated_fwd_kernel(const GatedScanParams p, const Chain q, float *ckpt, int saved) {
   __shared__ WaveSteps<V, NW> steps;
   __shared__ Ahead<V, NW> ahead;
@@ -49,9 +49,9 @@ __global__ __launch_bounds__(NW * 64, 4) void gated_fwd_kernel(const GatedScanPa
     const T *gr = static_cast<const T *>(p.gate_x) + b * p.gate_x_bs + from * p.gate_x_ls;
 #pragma unroll
     for (int j = 0; j < R; ++j) {  // past the row the last position again and again
-      ga[j] = at.template load<few.value>(ar);
-      gx[j] = at.template load<few.value>(gr);
-      x[j] = at.template load<few.value>(xr);
+      ga[j] = at.template load<few.value, STREAM >= 1>(ar);
+      gx[j] = at.template load<few.value, STREAM >= 1>(gr);
+      x[j] = at.template load<few.value, STREAM >= 1>(xr);
       const bool on = t0 + j + 1 < L;
       ar += on ? p.gate_a_ls : 0, gr += on ? p.gate_x_ls : 0, xr += on ? p.x_ls : 0;
     }
@@ -111,7 +111,7 @@ __global__ __launch_bounds__(NW * 64, 4) void gated_fwd_kernel(const GatedScanPa
 #pragma unroll
     for (int j = 0; j < R; ++j) {
       h = apply<with_edges.value>(pos[j], h);
-      if (j < rows) at.store(out, h);
+      if (j < rows) at.template store<STREAM >= 2>(out, h);
       out += p.out_ls;
       if constexpr (with_edges.value) {
         if (p.final_states && (seqs.last >> j & 1)) at.store_state(p.final_states + (int64_t)seqs.seq[j] * p.dim, h);
@@ -135,7 +135,7 @@ __global__ __launch_bounds__(NW * 64, 4) void gated_fwd_kernel(const GatedScanPa
 }
 
 // Tiles from the last one on: what enters a tile is a_t g_t of the position behind it.
-template <typename T, int V, bool WHOLE, bool PACKED, int R, int NW>
+template <typename T, int V, bool WHOLE, bool PACKED, int R, int NW, int STREAM>
 __global__ __launch_bounds__(NW * 64, NW > 4 ? 2 : 3) void gated_bwd_kernel(const GatedScanParams p, const Chain q, const float *ckpt, int saved, float *parts) {
   __shared__ WaveSteps<V, NW> steps, back;
   __shared__ Ahead<V, NW> ahead;
@@ -160,10 +160,10 @@ __global__ __launch_bounds__(NW * 64, NW > 4 ? 2 : 3) void gated_bwd_kernel(cons
     const T *dr = static_cast<const T *>(p.dout) + b * p.dout_bs + from * p.dout_ls;
 #pragma unroll
     for (int j = 0; j < R; ++j) {
-      ga[j] = at.template load<few.value>(ar);
-      gx[j] = at.template load<few.value>(gr);
-      x[j] = at.template load<few.value>(xr);
-      d[j] = at.template load<few.value>(dr);
+      ga[j] = at.template load<few.value, STREAM >= 1>(ar);
+      gx[j] = at.template load<few.value, STREAM >= 1>(gr);
+      x[j] = at.template load<few.value, STREAM >= 1>(xr);
+      d[j] = at.template load<few.value, STREAM >= 1>(dr);
       const bool on = t0 + j + 1 < L;
       ar += on ? p.gate_a_ls : 0, gr += on ? p.gate_x_ls : 0, xr += on ? p.x_ls : 0, dr += on ? p.dout_ls : 0;
     }
@@ -299,9 +299,9 @@ __global__ __launch_bounds__(NW * 64, NW > 4 ? 2 : 3) void gated_bwd_kernel(cons
         carry[e] = a[j][e] * g;
       }
       if (j < rows) {
-        at.store(dxr, dx);
-        at.store(dar, da);
-        at.store(dgr, dg);
+        at.template store<STREAM >= 2>(dxr, dx);
+        at.template store<STREAM >= 2>(dar, da);
+        at.template store<STREAM >= 2>(dgr, dg);
       }
       dxr -= p.dx_ls, dar -= p.dgate_a_ls, dgr -= p.dgate_x_ls;
       if constexpr (E) {
@@ -333,30 +333,41 @@ __global__ __launch_bounds__(NW * 64, NW > 4 ? 2 : 3) void gated_bwd_kernel(cons
 }
 
 // ------------------------------------------------------------------ host side
-// A pass's tiles of R positions per wave and NW waves, by its size.
+// How a pass is cut, by its size: tiles of R positions per wave and NW waves; whether rows stream past the caches
+// (0: no, 1: what is read, 2: what is written too).
+//   R, NW: kernels alone, us, bf16 -- forward at 777 x 1536 (156 tiles of 64 positions) 8 x 8 11.4, 16 x 8 12.7, at 2 x 2048 x 1536
+//   in fp32 (768) 34.4 and 31.4; backward there 8 x 8 52, 8 x 4 59, at 16384 x 1024 (2048 tiles) 87 and 96, at 4 x 2048 x 2560
+//   (2560 tiles) 102 and 97, at 8 x 4096 x 5120 776 and 616; 4 x 9 x 1536 4 x 8 4.6, 16 x 8 6.9.
+//   STREAM: with a pass over the results behind it, as a program has one -- forward and backward at 777 x 1536 0: 13.2 + 22.6, 1:
+//   14.3 + 22.8, 2: 14.7 + 23.5; at 4 x 2048 x 2560 (42 MB a tensor) 60.7 + 141, 60.1 + 138, 62.7 + 135; at 4 x 4096 x 5120 (168 MB)
+//   207 + 497, 197 + 486, 195 + 469.
 struct Form {
-  int r, nw;
+  int r, nw, stream;
 };
 int64_t chains_of(const GatedScanParams &p) { return (int64_t)p.batch * ((p.dim + kTileChannels - 1) / kTileChannels); }
 int64_t tiles_of(const GatedScanParams &p, int rows) { return chains_of(p) * (((int64_t)p.seqlen + rows - 1) / rows); }
+bool large(const GatedScanParams &p) {
+  return (int64_t)p.batch * p.seqlen * p.dim >= (int64_t)(64 << 20) / (p.dtype == MAMBA_F32 ? 4 : 2);
+}
 Form fwd_form(const GatedScanParams &p) {
-  if (p.seqlen <= 32) return {4, 8};
-  return tiles_of(p, 64) <= 512 ? Form{8, 8} : Form{16, 8};
+  if (p.seqlen <= 32) return {4, 8, 0};
+  return tiles_of(p, 64) <= 512 ? Form{8, 8, 0} : Form{16, 8, large(p) ? 2 : 1};
 }
 Form bwd_form(const GatedScanParams &p) {
-  if (p.seqlen <= 32) return {4, 8};
-  return tiles_of(p, 64) <= 2048 ? Form{8, 8} : Form{8, 4};
+  if (p.seqlen <= 32) return {4, 8, 0};
+  return tiles_of(p, 64) <= 2048 ? Form{8, 8, 1} : Form{8, 4, large(p) ? 2 : 1};
 }
-// f(R, NW) as compile-time values
+template <int N> using Int = std::integral_constant<int, N>;
+// f(R, NW, STREAM) as compile-time values
 template <typename F> int with_fwd_form(Form o, F f) {
-  if (o.r == 4) return f(std::integral_constant<int, 4>{}, std::integral_constant<int, 8>{});
-  if (o.r == 8) return f(std::integral_constant<int, 8>{}, std::integral_constant<int, 8>{});
-  return f(std::integral_constant<int, 16>{}, std::integral_constant<int, 8>{});
+  if (o.r == 4) return f(Int<4>{}, Int<8>{}, Int<0>{});
+  if (o.r == 8) return f(Int<8>{}, Int<8>{}, Int<0>{});
+  return o.stream == 1 ? f(Int<16>{}, Int<8>{}, Int<1>{}) : f(Int<16>{}, Int<8>{}, Int<2>{});
 }
 template <typename F> int with_bwd_form(Form o, F f) {
-  if (o.r == 4) return f(std::integral_constant<int, 4>{}, std::integral_constant<int, 8>{});
-  if (o.nw == 8) return f(std::integral_constant<int, 8>{}, std::integral_constant<int, 8>{});
-  return f(std::integral_constant<int, 8>{}, std::integral_constant<int, 4>{});
+  if (o.r == 4) return f(Int<4>{}, Int<8>{}, Int<0>{});
+  if (o.nw == 8) return f(Int<8>{}, Int<8>{}, Int<1>{});
+  return o.stream == 1 ? f(Int<8>{}, Int<4>{}, Int<1>{}) : f(Int<8>{}, Int<4>{}, Int<2>{});
 }
 
 // Tiles of one pass and what its chains need in memory: the tickets and words, cleared before the launch, lie at the
@@ -441,8 +452,8 @@ extern "C" int gated_scan_fwd(const GatedScanParams *p, mamba_stream_t stream) {
     if (const int rc = mamba_hip_zero(p->ckpt, plan.head, stream)) return rc;
   float *saved = reinterpret_cast<float *>(static_cast<char *>(p->ckpt) + plan.head);
   return with_types(*p, [&](auto t, auto whole, auto packed) {
-    return with_fwd_form(o, [&](auto r, auto nw) {
-      gated_fwd_kernel<decltype(t), kV, whole.value, packed.value, r.value, nw.value>
+    return with_fwd_form(o, [&](auto r, auto nw, auto stream_rows) {
+      gated_fwd_kernel<decltype(t), kV, whole.value, packed.value, r.value, nw.value, stream_rows.value>
           <<<dim3((unsigned)(plan.chains * plan.ntiles)), dim3(nw.value * 64), 0, static_cast<hipStream_t>(stream)>>>(
               *p, plan.chain(p->ckpt), saved, saved_states(*p));
       return hipGetLastError() == hipSuccess ? MAMBA_OK : MAMBA_E_LAUNCH;
@@ -459,8 +470,8 @@ extern "C" int gated_scan_bwd(const GatedScanParams *p, mamba_stream_t stream) {
   const float *saved = reinterpret_cast<const float *>(static_cast<const char *>(p->ckpt) + Plan(*p, fwd_form(*p)).head);
   float *parts = reinterpret_cast<float *>(static_cast<char *>(p->ws) + plan.head);
   const int rc = with_types(*p, [&](auto t, auto whole, auto packed) {
-    return with_bwd_form(o, [&](auto r, auto nw) {
-      gated_bwd_kernel<decltype(t), kV, whole.value, packed.value, r.value, nw.value>
+    return with_bwd_form(o, [&](auto r, auto nw, auto stream_rows) {
+      gated_bwd_kernel<decltype(t), kV, whole.value, packed.value, r.value, nw.value, stream_rows.value>
           <<<dim3((unsigned)(plan.chains * plan.ntiles)), dim3(nw.value * 64), 0, st>>>(*p, plan.chain(p->ws), saved, saved_states(*p), parts);
       return hipGetLastError() == hipSuccess ? MAMBA_OK : MAMBA_E_LAUNCH;
     });

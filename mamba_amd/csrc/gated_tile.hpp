@@ -67,7 +67,8 @@ template <typename T, int V, bool WHOLE> struct Lane {
     at = (uint32_t)from * sizeof(T);
     to = (uint32_t)c * sizeof(T);
   }
-  template <bool FEW = false> DEVI R load(const T *row) const {
+  // STREAM: past the caches' hold (the rows are read once, or written and not soon read)
+  template <bool FEW = false, bool STREAM = false> DEVI R load(const T *row) const {
     R r;
     const GLOBAL_AS char *p = (const GLOBAL_AS char *)row;
     if constexpr (FEW) {
@@ -82,7 +83,8 @@ template <typename T, int V, bool WHOLE> struct Lane {
       for (int i = 0; i < R::W; ++i) r.w[i] = R::HALF ? q[2 * i] | q[2 * i + 1] << 16 : q[i];
     } else {
       typedef typename Words<R::W, sizeof(T)>::type words;
-      const words v = *(const GLOBAL_AS words *)(p + at);
+      const GLOBAL_AS words *src = (const GLOBAL_AS words *)(p + at);
+      const words v = STREAM ? __builtin_nontemporal_load(src) : *src;
 #pragma unroll
       for (int i = 0; i < R::W; ++i) r.w[i] = v[i];
     }
@@ -108,7 +110,7 @@ template <typename T, int V, bool WHOLE> struct Lane {
       else f(std::false_type{});
     }
   }
-  DEVI void store(T *row, const Vec<V> &x) const {
+  template <bool STREAM = false> DEVI void store(T *row, const Vec<V> &x) const {
     typedef typename Words<R::W, sizeof(T)>::type words;
     GLOBAL_AS char *p = (GLOBAL_AS char *)row;
     words v;
@@ -119,7 +121,9 @@ template <typename T, int V, bool WHOLE> struct Lane {
       else v[i] = pack_f16(x.v[2 * i], x.v[2 * i + 1]);
     }
     if (n == V) {
-      *(GLOBAL_AS words *)(p + to) = v;
+      GLOBAL_AS words *dst = (GLOBAL_AS words *)(p + to);
+      if (STREAM) __builtin_nontemporal_store(v, dst);
+      else *dst = v;
     } else if (!WHOLE) {
 #pragma unroll
       for (int e = 0; e < V - 1; ++e)
