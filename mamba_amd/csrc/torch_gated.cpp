@@ -166,7 +166,6 @@ at::Tensor rows_of(const at::Tensor &t) {
   const at::Tensor r = t.dim() == 2 ? t : t.reshape({-1, t.size(-1)});
   return unit(r) ? r : r.contiguous();
 }
-at::Tensor shaped(const at::Tensor &t, at::IntArrayRef sizes) { return t.sizes() == sizes ? t : t.view(sizes); }
 
 void fill(NormBlockParams &p, const at::Tensor &x, const at::Tensor &residual, const at::Tensor &norm_w, const at::Tensor &next_w,
           const OptTensor &z, const OptTensor &scale, const OptTensor &norm_b, const OptTensor &next_b, const Block &o) {
@@ -178,14 +177,16 @@ void fill(NormBlockParams &p, const at::Tensor &x, const at::Tensor &residual, c
   p.x_rs = x.stride(0), p.z_rs = z ? z->stride(0) : 0, p.residual_rs = residual.stride(0);
 }
 
-// out, residual_out, the rows' statistics (undefined unless they are to be kept)
-std::tuple<at::Tensor, at::Tensor, at::Tensor> block_fwd(const at::Tensor &x, const at::Tensor &residual, const at::Tensor &norm_w,
-                                                         const at::Tensor &next_w, const OptTensor &z, const OptTensor &scale,
-                                                         const OptTensor &norm_b, const OptTensor &next_b, const Block &o, bool keep) {
+// out and residual_out in `sizes` (no views of rows: an output of several that is a view takes no in-place writes), the rows'
+// statistics (undefined unless they are to be kept)
+std::tuple<at::Tensor, at::Tensor, at::Tensor> block_fwd(at::IntArrayRef sizes, const at::Tensor &x, const at::Tensor &residual,
+                                                         const at::Tensor &norm_w, const at::Tensor &next_w, const OptTensor &z,
+                                                         const OptTensor &scale, const OptTensor &norm_b, const OptTensor &next_b,
+                                                         const Block &o, bool keep) {
   NormBlockParams p{};
   fill(p, x, residual, norm_w, next_w, z, scale, norm_b, next_b, o);
   c10::DeviceGuard guard(x.device());
-  at::Tensor out = at::empty({p.rows, p.dim}, x.options()), total = at::empty({p.rows, p.dim}, residual.options()), stats;
+  at::Tensor out = at::empty(sizes, x.options()), total = at::empty(sizes, residual.options()), stats;
   if (keep) stats = at::empty({p.rows, 4}, x.options().dtype(at::kFloat)), p.stats = stats.data_ptr<float>();
   p.out = out.data_ptr(), p.residual_out = total.data_ptr(), p.out_rs = p.residual_out_rs = p.dim;
   check_rc(norm_block_fwd(&p, stream_of(x.device())), "norm_block_fwd");
@@ -198,13 +199,13 @@ struct BlockNormFn : torch::autograd::Function<BlockNormFn> {
                                const OptTensor &next_b, const Block &o) {
     const at::Tensor x2 = rows_of(x), r2 = rows_of(residual);
     const OptTensor z2 = z ? OptTensor(rows_of(*z)) : std::nullopt;
-    auto [out, total, stats] = block_fwd(x2, r2, norm_w, next_w, z2, scale, norm_b, next_b, o, true);
+    auto [out, total, stats] = block_fwd(x.sizes(), x2, r2, norm_w, next_w, z2, scale, norm_b, next_b, o, true);
     ctx->save_for_backward({x2, r2, norm_w, next_w, tensor_or_none(z2), tensor_or_none(scale), tensor_or_none(norm_b),
                             tensor_or_none(next_b), stats});
     ctx->set_materialize_grads(false);
     ctx->saved_data["eps"] = o.eps, ctx->saved_data["scale"] = o.scale, ctx->saved_data["is_rms"] = o.is_rms;
     ctx->saved_data["shape"] = x.sizes().vec();
-    return {shaped(out, x.sizes()), shaped(total, x.sizes())};
+    return {out, total};
   }
   static variable_list backward(AutogradContext *ctx, variable_list grads) {
     variable_list g(9);
@@ -219,8 +220,8 @@ struct BlockNormFn : torch::autograd::Function<BlockNormFn> {
     c10::DeviceGuard guard(x.device());
     const at::Tensor dout = grads[0].defined() ? rows_of(grads[0]) : at::zeros(x.sizes(), x.options());
     const at::Tensor dsum = grads[1].defined() ? rows_of(grads[1]) : at::Tensor();
-    const at::Tensor dx = at::empty(x.sizes(), x.options()), dres = at::empty(residual.sizes(), residual.options());
-    const at::Tensor dz = z ? at::empty(x.sizes(), x.options()) : at::Tensor();
+    const at::Tensor dx = at::empty(shape, x.options()), dres = at::empty(shape, residual.options());
+    const at::Tensor dz = z ? at::empty(shape, x.options()) : at::Tensor();
     const int nsums = 2 + (scale ? 1 : 0) + (norm_b ? 1 : 0) + (next_b ? 1 : 0);
     const at::Tensor sums = at::empty({nsums, p.dim}, norm_w.options());
     p.stats = s[8].data_ptr<float>();
@@ -242,8 +243,8 @@ struct BlockNormFn : torch::autograd::Function<BlockNormFn> {
     const at::Tensor parts = at::empty({carried * p.nparts * p.dim}, x.options().dtype(at::kFloat));
     p.parts = parts.data_ptr<float>();
     check_rc(norm_block_bwd(&p, stream_of(x.device())), "norm_block_bwd");
-    g[0] = shaped(dx, shape), g[1] = shaped(dres, shape);
-    if (z) g[4] = shaped(dz, shape);
+    g[0] = dx, g[1] = dres;
+    if (z) g[4] = dz;
     return once(std::move(g), "block_norm");
   }
 };
@@ -272,9 +273,9 @@ pybind11::object block_norm(const at::Tensor &x, const at::Tensor &residual, con
     if (*t && !param(**t)) return no;
   const Block o{eps, scale_value, is_rms};
   if (!records(x, residual, norm_w, next_w, z, scale, norm_b, next_b)) {
-    auto [out, total, stats] = block_fwd(rows_of(x), rows_of(residual), norm_w, next_w, z ? OptTensor(rows_of(*z)) : std::nullopt, scale,
-                                         norm_b, next_b, o, false);
-    return pybind11::make_tuple(shaped(out, x.sizes()), shaped(total, x.sizes()));
+    auto [out, total, stats] = block_fwd(x.sizes(), rows_of(x), rows_of(residual), norm_w, next_w,
+                                         z ? OptTensor(rows_of(*z)) : std::nullopt, scale, norm_b, next_b, o, false);
+    return pybind11::make_tuple(out, total);
   }
   variable_list r = BlockNormFn::apply(x, residual, norm_w, next_w, z, scale, norm_b, next_b, o);
   return pybind11::make_tuple(r[0], r[1]);

@@ -42,13 +42,14 @@ class BlockNormFn(torch.autograd.Function):
         shape = x.shape
         x, residual, z = _rows(x), _rows(residual), _rows(z) if z is not None else None
         rows, dim = x.shape
-        out = torch.empty(rows, dim, dtype=x.dtype, device=x.device)
-        total = torch.empty(rows, dim, dtype=residual.dtype, device=x.device)
+        # in x's shape, no views of rows: an output of several that is a view takes no in-place writes
+        out = torch.empty(shape, dtype=x.dtype, device=x.device)
+        total = torch.empty(shape, dtype=residual.dtype, device=x.device)
         stats = torch.empty(rows, 4, dtype=torch.float32, device=x.device)
         if rows > 0:
             p = _params(x, residual, norm_weight, next_weight, z, scale, norm_bias, next_bias, eps, is_rms_norm)
             p.out, p.residual_out, p.stats = out.data_ptr(), total.data_ptr(), stats.data_ptr()
-            p.out_rs, p.residual_out_rs = out.stride(0), total.stride(0)
+            p.out_rs = p.residual_out_rs = dim
             with torch.cuda.device(x.device):
                 _lib.check(_lib.load().norm_block_fwd(p, _lib.current_stream(x.device)), "norm_block_fwd")
         ctx.save_for_backward(x, residual, norm_weight, next_weight, z, scale if isinstance(scale, torch.Tensor) else None,
@@ -56,7 +57,7 @@ class BlockNormFn(torch.autograd.Function):
         ctx.scale = None if isinstance(scale, torch.Tensor) else scale
         ctx.eps, ctx.is_rms_norm, ctx.shape = eps, is_rms_norm, shape
         ctx.set_materialize_grads(False)
-        return out.reshape(shape), total.reshape(shape)
+        return out, total
 
     @staticmethod
     @torch.autograd.function.once_differentiable
@@ -67,8 +68,8 @@ class BlockNormFn(torch.autograd.Function):
         rows, dim = x.shape
         dout = _rows(dout) if dout is not None else torch.zeros(rows, dim, dtype=x.dtype, device=x.device)
         dsum = _rows(dsum) if dsum is not None else None
-        dx, dresidual = torch.empty(rows, dim, dtype=x.dtype, device=x.device), torch.empty(rows, dim, dtype=residual.dtype, device=x.device)
-        dz = torch.empty(rows, dim, dtype=x.dtype, device=x.device) if z is not None else None
+        dx, dresidual = (torch.empty(ctx.shape, dtype=t.dtype, device=x.device) for t in (x, residual))
+        dz = torch.empty(ctx.shape, dtype=x.dtype, device=x.device) if z is not None else None
         given = [(n, t) for n, t in (("dnorm_weight", norm_weight), ("dnext_weight", next_weight), ("dscale", scale),
                                      ("dnorm_bias", norm_bias), ("dnext_bias", next_bias)) if t is not None]
         sums = (torch.empty if rows > 0 else torch.zeros)(len(given), dim, dtype=norm_weight.dtype, device=x.device)
@@ -79,7 +80,7 @@ class BlockNormFn(torch.autograd.Function):
             p.stats = stats.data_ptr()
             p.dout, p.dsum, p.dx, p.dresidual, p.dz = dout.data_ptr(), _lib.ptr(dsum), dx.data_ptr(), dresidual.data_ptr(), _lib.ptr(dz)
             p.dout_rs, p.dsum_rs = dout.stride(0), dsum.stride(0) if dsum is not None else 0
-            p.dx_rs, p.dresidual_rs, p.dz_rs = dx.stride(0), dresidual.stride(0), dz.stride(0) if dz is not None else 0
+            p.dx_rs = p.dresidual_rs = p.dz_rs = dim
             for n, g in grads.items():
                 setattr(p, n, g.data_ptr())
             with torch.cuda.device(x.device):
@@ -89,9 +90,8 @@ class BlockNormFn(torch.autograd.Function):
                 parts = torch.empty(nsums, p.nparts, dim, dtype=torch.float32, device=x.device)
                 p.parts = parts.data_ptr()
                 _lib.check(lib.norm_block_bwd(p, _lib.current_stream(x.device)), "norm_block_bwd")
-        og = lambda t: t.reshape(ctx.shape) if t is not None else None
-        return (og(dx), og(dresidual), grads["dnorm_weight"], grads["dnext_weight"], og(dz), grads.get("dscale"),
-                grads.get("dnorm_bias"), grads.get("dnext_bias"), None, None)
+        return (dx, dresidual, grads["dnorm_weight"], grads["dnext_weight"], dz, grads.get("dscale"), grads.get("dnorm_bias"),
+                grads.get("dnext_bias"), None, None)
 
 
 def block_norm_fn(x, residual, norm_weight, next_weight, z=None, scale=None, norm_bias=None, next_bias=None, eps=1e-5,
