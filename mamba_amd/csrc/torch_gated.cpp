@@ -203,7 +203,7 @@ struct BlockNormFn : torch::autograd::Function<BlockNormFn> {
     ctx->save_for_backward({x2, r2, norm_w, next_w, tensor_or_none(z2), tensor_or_none(scale), tensor_or_none(norm_b),
                             tensor_or_none(next_b), stats});
     ctx->set_materialize_grads(false);
-    ctx->saved_data["eps"] = o.eps, ctx->saved_data["scale"] = o.scale, ctx->saved_data["is_rms"] = o.is_rms;
+    ctx->saved_data["o"] = std::vector<double>{o.eps, o.scale, (double)o.is_rms};
     ctx->saved_data["shape"] = x.sizes().vec();
     return {out, total};
   }
@@ -213,7 +213,8 @@ struct BlockNormFn : torch::autograd::Function<BlockNormFn> {
     const variable_list s = ctx->get_saved_variables();
     const at::Tensor &x = s[0], &residual = s[1], &norm_w = s[2];
     const OptTensor z = opt(s[4]), scale = opt(s[5]), norm_b = opt(s[6]), next_b = opt(s[7]);
-    const Block o{ctx->saved_data["eps"].toDouble(), ctx->saved_data["scale"].toDouble(), ctx->saved_data["is_rms"].toBool()};
+    const std::vector<double> v = ctx->saved_data["o"].toDoubleVector();
+    const Block o{v[0], v[1], v[2] != 0.0};
     const std::vector<int64_t> shape = ctx->saved_data["shape"].toIntVector();
     NormBlockParams p{};
     fill(p, x, residual, norm_w, s[3], z, scale, norm_b, next_b, o);
@@ -223,7 +224,7 @@ struct BlockNormFn : torch::autograd::Function<BlockNormFn> {
     const at::Tensor dx = at::empty(shape, x.options()), dres = at::empty(shape, residual.options());
     const at::Tensor dz = z ? at::empty(shape, x.options()) : at::Tensor();
     const int nsums = 2 + (scale ? 1 : 0) + (norm_b ? 1 : 0) + (next_b ? 1 : 0);
-    const at::Tensor sums = at::empty({nsums, p.dim}, norm_w.options());
+    const std::vector<at::Tensor> sums = at::empty({nsums, p.dim}, norm_w.options()).unbind(0);
     p.stats = s[8].data_ptr<float>();
     p.dout = dout.data_ptr(), p.dout_rs = dout.stride(0);
     if (dsum.defined()) p.dsum = dsum.data_ptr(), p.dsum_rs = dsum.stride(0);
@@ -231,7 +232,7 @@ struct BlockNormFn : torch::autograd::Function<BlockNormFn> {
     if (z) p.dz = dz.data_ptr();
     int n = 0;
     auto sum = [&](at::Tensor &grad) -> void * {
-      grad = sums.select(0, n++);
+      grad = sums[n++];
       return grad.data_ptr();
     };
     p.dnorm_weight = sum(g[2]), p.dnext_weight = sum(g[3]);
