@@ -19,6 +19,11 @@ DEVI float softplus_exact(float x) {
   return x <= 20.f ? r : x;
 }
 
+// Factors of a state are positive; one that underflows is taken as the least normal number, so that an infinite state stays infinite
+// and 0 is free as a mark.  (A finite state times kTiny is gone all the same; a NaN stays one.)
+constexpr float kTiny = 1.17549435e-38f;
+DEVI float not_zero(float a) { return __builtin_elementwise_maximum(a, kTiny); }
+
 // One position's gates from kr's factor k and k2 = -k log2(e): r, i, a and m^2 = 1 - a^2.
 //   1 - exp(-2 w) = 2 exp(-w) sinh(w), w = k r: no cancellation where a is near 1, and its series needs two terms below
 // w = 0.25 (the next one is 5e-8 of the sum); from there on 1 - a^2 as it stands.
@@ -30,13 +35,17 @@ struct Gates {
     r = sigmoid_f(ga);
     i = sigmoid_f(gx);
     const float w = k * r, w2 = w * w;
-    a = __builtin_amdgcn_exp2f(k2 * r);
+    a = not_zero(__builtin_amdgcn_exp2f(k2 * r));
     const float s = __builtin_fmaf(w2, __builtin_fmaf(w2, 1.f / 60.f, 1.f / 3.f), 2.f);
-    m2 = w < 0.25f ? a * w * s : __builtin_fmaf(-a, a, 1.f);
+    const float near1 = a * w * s, else_ = __builtin_fmaf(-a, a, 1.f);  // both are formed: no branch
+    m2 = w < 0.25f ? near1 : else_;
   }
   DEVI float m() const { return __builtin_amdgcn_sqrtf(m2); }
   // 1 / m, 0 where m is 0 (a gate shut to the last bit, a decay of 0): r / m tends to 0 there like sqrt(r)
-  DEVI float im() const { return m2 > 0.f ? __builtin_amdgcn_rsqf(m2) : 0.f * m2; }  // (a NaN stays one)
+  DEVI float im() const {
+    const float root = __builtin_amdgcn_rsqf(m2);  // (of a NaN one)
+    return m2 == 0.f ? 0.f : root;
+  }
 };
 
 }  // namespace

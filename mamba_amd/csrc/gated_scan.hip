@@ -65,17 +65,16 @@ __global__ __launch_bounds__(NW * 64, 4) void gated_fwd_kernel(const GatedScanPa
 #pragma unroll
     for (int e = 0; e < V; ++e) {
       const Gates g(at.get(ga[j], e), at.get(gx[j], e), rate.k[e], rate.k2[e]);
-      pos[j].a[e] = PACKED ? fmaxf(g.a, kTiny) : g.a;
+      pos[j].a[e] = g.a;
       pos[j].b[e] = g.m() * g.i * at.get(x[j], e);
     }
     if (!PACKED && j >= rows) pos[j] = no_step<V>();
-    own = then<false>(own, pos[j]);
+    own = with(own, pos[j]);
   }
+  own = kept(own);
   // a wave with an edge of a sequence among its positions, or with some outside of all: the others never branch
   const bool edges = PACKED && seqs.edges();
   if constexpr (PACKED) {
-#pragma unroll
-    for (int e = 0; e < V; ++e) own.a[e] = fmaxf(own.a[e], kTiny);
     if (edges) {
       own = no_step<V>();
 #pragma unroll
@@ -196,7 +195,7 @@ __global__ __launch_bounds__(NW * 64, NW > 4 ? 2 : 3) void gated_bwd_kernel(cons
     for (int e = 0; e < V; ++e) {
       const Gates g(at.get(ga[j], e), at.get(gx[j], e), rate.k[e], rate.k2[e]);
       const float im = g.im();
-      a[j][e] = PACKED ? fmaxf(g.a, kTiny) : g.a;
+      a[j][e] = g.a;
       r[j][e] = g.r, i[j][e] = g.i, m[j][e] = g.m2 * im, f[j][e] = g.r * im;
     }
     if (!PACKED && j >= rows) {  // a position past the row hands everything on
@@ -227,7 +226,7 @@ __global__ __launch_bounds__(NW * 64, NW > 4 ? 2 : 3) void gated_bwd_kernel(cons
           s.a = vec_of<V>(0.f);
         }
       }
-      own = then<E>(own, s);
+      own = E ? then<true>(own, s) : with(own, s);
     }
 #pragma unroll
     for (int j = R - 1; j >= 0; --j) {
@@ -239,15 +238,14 @@ __global__ __launch_bounds__(NW * 64, NW > 4 ? 2 : 3) void gated_bwd_kernel(cons
       }
 #pragma unroll
       for (int e = 0; e < V; ++e) {
-        rev.a[e] = cut ? 0.f : factor1<E>(rev.a[e], a[j][e]);
+        rev.a[e] = cut ? 0.f : E ? factor1<true>(rev.a[e], a[j][e]) : rev.a[e] * a[j][e];
         rev.b[e] = a[j][e] * (rev.b[e] + at.get(d[j], e));
       }
     }
-    if constexpr (PACKED && !E) {
-#pragma unroll
-      for (int e = 0; e < V; ++e) own.a[e] = fmaxf(own.a[e], kTiny), rev.a[e] = fmaxf(rev.a[e], kTiny);
-    }
+    if constexpr (!E) own = kept(own), rev = kept(rev);
   });
+#pragma unroll
+  for (int j = 0; j < R; ++j) x[j].anew(), d[j].anew();
   steps.put(wave, lane, own);
   back.put(wave, lane, rev);
   lds_barrier();
@@ -400,9 +398,11 @@ bool shapes_ok(const GatedScanParams *p) {
   if (!(p->rate >= 0.f && p->rate <= 3.4e38f)) return false;
   return p->dtype >= MAMBA_F32 && p->dtype <= MAMBA_F16 && p->decay_dtype >= MAMBA_F32 && p->decay_dtype <= MAMBA_F16;
 }
-// positions, tiles and workgroups are counted in 32 bits
+// positions and tiles are counted in 32 bits, and so are the threads of a launch
 bool counts_fit(const GatedScanParams &p) {
-  return p.seqlen <= 0x7fffffff - 4096 && p.nseq <= 0x7fffffff - 64 && p.dim <= 0x7fffffff / 8 && tiles_of(p, 32) <= 0x7fffffff;
+  if (p.seqlen > 0x7fffffff - 4096 || p.nseq > 0x7fffffff - 64 || p.dim > 0x7fffffff / 8) return false;
+  const Form f = fwd_form(p), b = bwd_form(p);
+  return tiles_of(p, f.r * f.nw) * f.nw * 64 <= 0xffffffffll && tiles_of(p, b.r * b.nw) * b.nw * 64 <= 0xffffffffll;
 }
 int check(const GatedScanParams *p, bool bwd) {
   if (!shapes_ok(p)) return MAMBA_E_BADARG;

@@ -42,6 +42,14 @@ template <typename T, int V> struct Raw {
 #pragma unroll
     for (int i = 0; i < W; ++i) w[i] = 0;
   }
+  // From here on its values are formed anew: kept since they were formed first they take twice the registers of the words.  (The
+  // backward kernel spilled: 538 us at 8 x 4096 x 5120, now 512.)
+  DEVI void anew() {
+    if constexpr (HALF) {
+#pragma unroll
+      for (int i = 0; i < W; ++i) asm("" : "+v"(w[i]));
+    }
+  }
   DEVI float get(int e) const {
     if constexpr (!HALF) return __builtin_bit_cast(float, w[e]);
     else if constexpr (DT<T>::id == MAMBA_BF16) return e & 1 ? bf16_hi(w[e / 2]) : bf16_lo(w[e / 2]);
@@ -144,10 +152,7 @@ template <typename T, int V, bool WHOLE> struct Lane {
 };
 
 // The step of a run of positions: h -> a h + b per channel.
-// RESETS: a factor of exactly 0 marks a run in which a sequence starts; nothing before it counts, whatever it is.  The
-// decays of positions are kept from underflowing to that (a state times kTiny is gone all the same, but an infinity or a
-// NaN in the sequence stays one).
-constexpr float kTiny = 1.17549435e-38f;
+// RESETS: a factor of exactly 0 marks a run in which a sequence starts; nothing before it counts, whatever it is.
 template <int V> struct Step {
   Vec<V> a, b;
 };
@@ -157,15 +162,27 @@ template <bool RESETS> DEVI float apply1(float a, float b, float h) {
   return RESETS && a == 0.f ? b : r;
 }
 template <bool RESETS> DEVI float factor1(float a, float next) {
-  const float r = a * next;
-  if (!RESETS) return r;
-  return a == 0.f || next == 0.f ? 0.f : fmaxf(r, kTiny);
+  const float r = not_zero(a * next);
+  return RESETS && (a == 0.f || next == 0.f) ? 0.f : r;
 }
 template <bool RESETS, int V> DEVI Vec<V> apply(const Step<V> &s, const Vec<V> &h) {
   Vec<V> r;
 #pragma unroll
   for (int e = 0; e < V; ++e) r[e] = apply1<RESETS>(s.a[e], s.b[e], h[e]);
   return r;
+}
+// s with a position behind it that resets nothing; its factor may underflow to 0 on the way, `kept` makes that good at the end
+template <int V> DEVI Step<V> with(const Step<V> &s, const Step<V> &pos) {
+  Step<V> r;
+#pragma unroll
+  for (int e = 0; e < V; ++e) r.a[e] = s.a[e] * pos.a[e];
+  r.b = apply<false>(pos, s.b);
+  return r;
+}
+template <int V> DEVI Step<V> kept(Step<V> s) {
+#pragma unroll
+  for (int e = 0; e < V; ++e) s.a[e] = not_zero(s.a[e]);
+  return s;
 }
 template <bool RESETS, int V> DEVI Step<V> then(const Step<V> &s, const Step<V> &next) {
   Step<V> r;

@@ -244,3 +244,28 @@ def test_two_graphs_at_once():
     torch.cuda.synchronize()
     for (_, out), w in zip(graphs, want):
         assert torch.equal(out, w)
+
+
+@pytest.mark.parametrize("which", range(4))
+@pytest.mark.parametrize("value", [float("nan"), float("inf")])
+def test_in_packed_sequences_no_number_goes_as_far_as_in_rows_of_their_own(which, value):
+    """A NaN or an infinity at one position: packed and alone the same results and gradients are no numbers, and the other
+    sequences' are untouched."""
+    from mamba_amd.ops.gated_linear_scan import gated_linear_scan_fn
+    cu = [0, 40, 190, 191, 300]
+    g = torch.Generator(device="cuda").manual_seed(0)
+    tensors = [torch.randn(1, 300, 6, device="cuda", generator=g) for _ in range(4)]
+    for at, channel in ((5, 0), (60, 1), (189, 2), (190, 3), (191, 4)):
+        tensors[which][0, at, channel] = value
+
+    def run(ts, bounds):
+        leaves = [t.clone().requires_grad_() for t in ts[:3]]
+        out, final = gated_linear_scan_fn(*leaves, _fixed(8, 6), return_final_states=True, cu_seqlens=bounds)
+        return [out, final, *torch.autograd.grad([out, final], leaves, [ts[3], torch.ones_like(final)])]
+
+    packed = run(tensors, torch.tensor(cu, dtype=torch.int32, device="cuda"))
+    alone = [run([t[:, a:b] for t in tensors], None) for a, b in zip(cu, cu[1:])]
+    for n, got in enumerate(packed):
+        want = torch.cat([a[n] for a in alone], 0 if n == 1 else 1)
+        assert torch.equal(got.isnan(), want.isnan()) and torch.equal(got.isinf(), want.isinf())
+        torch.testing.assert_close(got, want, rtol=2e-4, atol=2e-5, equal_nan=True)

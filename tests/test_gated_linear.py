@@ -149,3 +149,12 @@ def test_c_entry_points_refuse_what_they_do_not_serve():
     assert lib.norm_block_fwd(p, None) == -2
     p.dim, p.dtype, p.res_dtype = 4, 1, 2      # a bf16 block on an fp16 stream
     assert lib.norm_block_fwd(p, None) == -2
+
+
+def test_more_workgroups_than_a_launch_takes():
+    lib = _lib.load()
+    p = _filled(_lib.GatedScanParams, **SCAN)
+    p.batch, p.seqlen, p.dim = 2 ** 23 - 1, 1, 1
+    assert lib.gated_scan_ckpt_bytes(p) > 0 and lib.gated_scan_bwd_ws_bytes(p) > 0
+    p.batch += 1                                # 2^32 threads
+    assert lib.gated_scan_ckpt_bytes(p) == lib.gated_scan_bwd_ws_bytes(p) == lib.gated_scan_fwd(p, None) == lib.gated_scan_bwd(p, None) == -2
