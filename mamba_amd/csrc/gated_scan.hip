@@ -4,8 +4,9 @@
 // and its gradients, with g_t = dout_t + a_{t+1} g_{t+1}:
 //   dx = g m i,  dgate_x = dx x (1 - i),  dgate_a = k (1 - r) e,  ddecay = rate sigmoid(decay) sum e,
 //   e = g a (a i x r / m - r h_{t-1}),  dinitial = a g at the first position
-// The forward pass moves 4 tensors and the backward pass 7: both are bound by memory (about 80 vector slots per element
-// backward, half of them the six quarter-rate instructions of a position, are below half of the time the bytes take).
+// The forward pass moves 4 tensors and the backward pass 7: both are bound by memory.  8 x 4096 x 5120 bf16: forward 270 us, 5.0 TB/s,
+// backward 513 us, 4.6 TB/s, where a copy of long rows reaches 6.2 and a bare pass in this pattern (tiles of 256-byte pieces of rows, 3
+// tensors in and 1 out, or 4 and 3) 5.1 and 5.0.  (Three vector instructions fewer per element backward left its time as it was.)
 // gated_tile.hpp says how a row is cut.  The forward pass leaves the state that enters every tile of the backward
 // pass, which then forms its own states again: one float per tile and channel instead of the states in 32 bits.
 #include "gated_tile.hpp"
@@ -338,33 +339,46 @@ __global__ __launch_bounds__(NW * 64, NW > 4 ? 2 : 3) void gated_bwd_kernel(cons
 //   (2560 tiles) 102 and 97, at 8 x 4096 x 5120 776 and 616; 4 x 9 x 1536 4 x 8 4.6, 16 x 8 6.9.
 //   STREAM: with a pass over the results behind it, as a program has one -- forward and backward at 777 x 1536 0: 13.2 + 22.6, 1:
 //   14.3 + 22.8, 2: 14.7 + 23.5; at 4 x 2048 x 2560 (42 MB a tensor) 60.7 + 141, 60.1 + 138, 62.7 + 135; at 4 x 4096 x 5120 (168 MB)
-//   207 + 497, 197 + 486, 195 + 469.
+//   207 + 497, 197 + 486, 195 + 469.  Rows that do not lie on 64 bytes never: two groups of channels share a line, which is gone by
+//   the second -- kernels alone, 0 and 2 at 4 x 4096 x 5121 190 + 386 and 205 + 423, x 5128 175 + 357 and 193 + 389, x 5152 (rows on 64
+//   bytes, not 128) 152 + 306 and 153 + 287.
 struct Form {
   int r, nw, stream;
 };
 int64_t chains_of(const GatedScanParams &p) { return (int64_t)p.batch * ((p.dim + kTileChannels - 1) / kTileChannels); }
 int64_t tiles_of(const GatedScanParams &p, int rows) { return chains_of(p) * (((int64_t)p.seqlen + rows - 1) / rows); }
-bool large(const GatedScanParams &p) {
-  return (int64_t)p.batch * p.seqlen * p.dim >= (int64_t)(64 << 20) / (p.dtype == MAMBA_F32 ? 4 : 2);
+int streams(const GatedScanParams &p, bool bwd) {
+  const int size = p.dtype == MAMBA_F32 ? 4 : 2;
+  auto at = [&](const void *t, int64_t bs, int64_t ls) { return (uint64_t)reinterpret_cast<uintptr_t>(t) | (uint64_t)((bs | ls) * size); };
+  uint64_t all = at(p.x, p.x_bs, p.x_ls) | at(p.gate_a, p.gate_a_bs, p.gate_a_ls) | at(p.gate_x, p.gate_x_bs, p.gate_x_ls);
+  if (bwd)
+    all |= at(p.dout, p.dout_bs, p.dout_ls) | at(p.dx, p.dx_bs, p.dx_ls) | at(p.dgate_a, p.dgate_a_bs, p.dgate_a_ls) |
+           at(p.dgate_x, p.dgate_x_bs, p.dgate_x_ls);
+  else
+    all |= at(p.out, p.out_bs, p.out_ls);
+  if (all % 64 != 0) return 0;
+  return (int64_t)p.batch * p.seqlen * p.dim >= (int64_t)(64 << 20) / size ? 2 : 1;
 }
 Form fwd_form(const GatedScanParams &p) {
   if (p.seqlen <= 32) return {4, 8, 0};
-  return tiles_of(p, 64) <= 512 ? Form{8, 8, 0} : Form{16, 8, large(p) ? 2 : 1};
+  return tiles_of(p, 64) <= 512 ? Form{8, 8, 0} : Form{16, 8, streams(p, false)};
 }
 Form bwd_form(const GatedScanParams &p) {
   if (p.seqlen <= 32) return {4, 8, 0};
-  return tiles_of(p, 64) <= 2048 ? Form{8, 8, 1} : Form{8, 4, large(p) ? 2 : 1};
+  return tiles_of(p, 64) <= 2048 ? Form{8, 8, min(streams(p, true), 1)} : Form{8, 4, streams(p, true)};
 }
 template <int N> using Int = std::integral_constant<int, N>;
 // f(R, NW, STREAM) as compile-time values
 template <typename F> int with_fwd_form(Form o, F f) {
   if (o.r == 4) return f(Int<4>{}, Int<8>{}, Int<0>{});
   if (o.r == 8) return f(Int<8>{}, Int<8>{}, Int<0>{});
+  if (o.stream == 0) return f(Int<16>{}, Int<8>{}, Int<0>{});
   return o.stream == 1 ? f(Int<16>{}, Int<8>{}, Int<1>{}) : f(Int<16>{}, Int<8>{}, Int<2>{});
 }
 template <typename F> int with_bwd_form(Form o, F f) {
   if (o.r == 4) return f(Int<4>{}, Int<8>{}, Int<0>{});
-  if (o.nw == 8) return f(Int<8>{}, Int<8>{}, Int<1>{});
+  if (o.nw == 8) return o.stream == 0 ? f(Int<8>{}, Int<8>{}, Int<0>{}) : f(Int<8>{}, Int<8>{}, Int<1>{});
+  if (o.stream == 0) return f(Int<8>{}, Int<4>{}, Int<0>{});
   return o.stream == 1 ? f(Int<8>{}, Int<4>{}, Int<1>{}) : f(Int<8>{}, Int<4>{}, Int<2>{});
 }
 
