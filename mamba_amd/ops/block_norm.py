@@ -129,6 +129,8 @@ def block_norm_fn(x, residual, norm_weight, next_weight, z=None, scale=None, nor
     dim = x.shape[-1]
     if dim < 1 or dim > 32768:
         raise RuntimeError(f"{what}: rows of 1 to 32768 channels are served, got {dim}")
+    if x.numel() // dim > 2 ** 31 - 1:
+        raise RuntimeError(f"{what}: rows are counted in 32 bits, got {x.numel() // dim}")
     params = dict(norm_weight=norm_weight, next_weight=next_weight, scale=tensor_scale, norm_bias=norm_bias, next_bias=next_bias)
     for name, t in params.items():
         if t is not None and (tuple(t.shape) != (dim,) or t.dtype not in _lib.DTYPE_CODE):

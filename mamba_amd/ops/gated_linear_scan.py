@@ -39,6 +39,16 @@ def _one_device(what, first, *others):
             raise RuntimeError(f"{what}: all tensors must be on {first.device}, got one on {t.device}")
 
 
+def _check_sizes(what, *sizes):
+    if max(sizes) > 2 ** 31 - 1:
+        raise RuntimeError(f"{what}: sizes are counted in 32 bits, got {max(sizes)}")
+
+
+def _int32(t, low, high):
+    """Bounds or row numbers in 32 bits; 64-bit ones are first taken to [low, high], so that none turns into another."""
+    return (t if t.dtype == torch.int32 else t.clamp(low, high).to(torch.int32)).contiguous()
+
+
 def _params(x, gate_a, gate_x, decay, initial_states, cu_seqlens, rate):
     p = _lib.GatedScanParams()
     p.batch, p.seqlen, p.dim = x.shape
@@ -144,6 +154,7 @@ def gated_linear_scan_fn(x, gate_a, gate_x, decay, rate=8.0, initial_states=None
     if x.dim() != 3 or x.dtype not in _lib.DTYPE_CODE:
         raise RuntimeError(f"{what}: x must be (batch, seqlen, dim) in fp32, fp16 or bf16")
     batch, seqlen, dim = x.shape
+    _check_sizes(what, batch, seqlen, dim)
     for name, t in (("gate_a", gate_a), ("gate_x", gate_x)):
         if t.shape != x.shape:
             raise RuntimeError(f"{what}: {name} must have x's shape {tuple(x.shape)}, got {tuple(t.shape)}")
@@ -161,7 +172,7 @@ def gated_linear_scan_fn(x, gate_a, gate_x, decay, rate=8.0, initial_states=None
     _lib.require_gpu(x, gate_a, gate_x, decay, initial_states, cu_seqlens)
     _one_device(what, x, gate_a, gate_x, decay, initial_states, cu_seqlens)
     if cu_seqlens is not None:
-        cu_seqlens = cu_seqlens.to(torch.int32).contiguous()
+        cu_seqlens = _int32(cu_seqlens, 0, seqlen)
     if initial_states is not None:
         initial_states = initial_states.float().contiguous()
     out, final = GatedLinearScanFn.apply(x, gate_a.to(x.dtype), gate_x.to(x.dtype), decay.contiguous(), initial_states,
@@ -190,6 +201,7 @@ def gated_linear_state_update(state, x, gate_a, gate_x, decay, rate=8.0, state_b
     if x.dim() != 2 or state.dim() != 2 or state.shape[1] != x.shape[1]:
         raise RuntimeError(f"{what}: state must be (rows, dim) and x (batch, dim)")
     batch, dim = x.shape
+    _check_sizes(what, batch, dim, state.shape[0])
     if state_batch_indices is None and state.shape[0] < batch:
         raise RuntimeError(f"{what}: state has {state.shape[0]} rows for a batch of {batch} and no state_batch_indices")
     for name, t in (("gate_a", gate_a), ("gate_x", gate_x)):
@@ -199,6 +211,8 @@ def gated_linear_state_update(state, x, gate_a, gate_x, decay, rate=8.0, state_b
         raise RuntimeError(f"{what}: x and state must be fp32, fp16 or bf16")
     if state.stride(1) != 1 and dim > 1:
         raise RuntimeError(f"{what}: state must have unit channel stride (it is updated in place)")
+    if state.stride(0) < dim and state.shape[0] > 1:
+        raise RuntimeError(f"{what}: state's rows must not overlap (they are updated in place)")
     _check_decay(what, decay, dim, x.device)
     rate = _check_rate(what, rate)
     if state_batch_indices is not None:
@@ -207,7 +221,7 @@ def gated_linear_state_update(state, x, gate_a, gate_x, decay, rate=8.0, state_b
     _lib.require_gpu(state, x, gate_a, gate_x, decay, state_batch_indices)
     _one_device(what, x, state, gate_a, gate_x, decay, state_batch_indices)
     if state_batch_indices is not None:
-        state_batch_indices = state_batch_indices.to(torch.int32).contiguous()
+        state_batch_indices = _int32(state_batch_indices, -1, 2 ** 31 - 1)
     out = torch.empty(batch, dim, dtype=x.dtype, device=x.device)
     if out.numel() == 0:
         return out

@@ -269,3 +269,19 @@ def test_in_packed_sequences_no_number_goes_as_far_as_in_rows_of_their_own(which
         want = torch.cat([a[n] for a in alone], 0 if n == 1 else 1)
         assert torch.equal(got.isnan(), want.isnan()) and torch.equal(got.isinf(), want.isinf())
         torch.testing.assert_close(got, want, rtol=2e-4, atol=2e-5, equal_nan=True)
+
+
+def test_row_numbers_of_64_bits_turn_into_no_others():
+    from mamba_amd.ops.gated_linear_scan import gated_linear_scan_fn, gated_linear_state_update
+    args = [t[:, :3].reshape(6, 48) for t in _operands()] + [_fixed(0, 2, 90, 48)[:, :3].reshape(6, 48), _fixed(1, 48)]
+    rows = [1, -1, 2 ** 32, 2 ** 32 + 2, 2 ** 31, -(2 ** 32) + 3]
+    states = [_fixed(2, 5, 48).clone() for _ in range(2)]
+    outs = [gated_linear_state_update(s, *args, state_batch_indices=torch.tensor(r, dtype=d, device="cuda"))
+            for s, r, d in zip(states, ([1] + [-1] * 5, rows), (torch.int32, torch.int64))]
+    assert torch.equal(*outs) and torch.equal(*states)
+    x, z = (t[:1] for t in _operands())
+    outs = [gated_linear_scan_fn(x, z, _fixed(0, 2, 90, 48)[:1], _fixed(1, 48), cu_seqlens=torch.tensor(c, dtype=d, device="cuda"))
+            for c, d in (([0, 7, 90], torch.int32), ([-(2 ** 32), 7, 2 ** 32 + 5], torch.int64))]
+    assert torch.equal(*outs)
+    with pytest.raises(RuntimeError, match="must not overlap"):
+        gated_linear_state_update(_fixed(2, 5, 48)[:1].expand(6, 48), *args)

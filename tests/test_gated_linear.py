@@ -158,3 +158,23 @@ def test_more_workgroups_than_a_launch_takes():
     assert lib.gated_scan_ckpt_bytes(p) > 0 and lib.gated_scan_bwd_ws_bytes(p) > 0
     p.batch += 1                                # 2^32 threads
     assert lib.gated_scan_ckpt_bytes(p) == lib.gated_scan_bwd_ws_bytes(p) == lib.gated_scan_fwd(p, None) == lib.gated_scan_bwd(p, None) == -2
+
+
+BIG = torch.zeros(1, dtype=torch.bfloat16)
+
+
+@pytest.mark.parametrize("call", [
+    lambda: gated_linear_scan_fn(*[BIG.expand(2 ** 31, 1, 1)] * 3, BIG),
+    lambda: gated_linear_scan_fn(*[BIG.expand(1, 2 ** 31, 1)] * 3, BIG),
+    lambda: gated_linear_state_update(torch.zeros(1, 1), *[BIG.expand(2 ** 31, 1)] * 3, BIG, state_batch_indices=BIG),
+    lambda: block_norm_fn(*[BIG.expand(2 ** 31, 1)] * 2, BIG, BIG)])
+def test_sizes_beyond_32_bits(call):
+    with pytest.raises(RuntimeError, match="counted in 32 bits"):
+        call()
+
+
+def test_overlapping_state_rows():
+    with pytest.raises(RuntimeError, match="must not overlap"):
+        _step(state=Z(1, 4).expand(3, 4))
+    with pytest.raises(RuntimeError, match="must not overlap"):
+        _step(state=Z(9).as_strided((3, 4), (2, 1)))
