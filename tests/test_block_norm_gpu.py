@@ -49,12 +49,12 @@ def _check(t, rms, with_dsum=True, eps=1e-5):
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("rows,dim", [(1, 1), (3, 2), (1, 7), (5, 8), (2, 63), (4, 64), (1, 100), (9, 256), (3, 257), (2, 511), (7, 512),
                                       (2, 520), (3, 768), (2, 1001), (5, 1024), (1, 1032), (2, 2048), (3, 2560), (1, 4096), (2, 4104),
-                                      (2, 5121), (1, 8192), (2, 8200), (1, 10000), (1, 32768)])
+                                      (2, 5121), (3, 6144), (2, 6152), (1, 8192), (2, 8200), (1, 10000), (1, 32768)])
 def test_sizes(rows, dim, dtype, rms):
     _check(_inputs((rows, dim), dtype, seed=dim), rms)
 
 
-@pytest.mark.parametrize("rows,dim", [(1100, 64), (700, 520), (5000, 8), (1500, 130), (300, 2560), (2100, 768)])
+@pytest.mark.parametrize("rows,dim", [(1100, 64), (700, 520), (5000, 8), (1500, 130), (300, 2560), (2100, 768), (600, 6144), (600, 6152), (900, 8192)])
 def test_many_rows(rows, dim):
     _check(_inputs((rows, dim), torch.bfloat16, stream=torch.float32, seed=rows), True)
 
