@@ -5,7 +5,7 @@
 //   dx = g m i,  dgate_x = dx x (1 - i),  dgate_a = k (1 - r) e,  ddecay = rate sigmoid(decay) sum e,
 //   e = g a (a i x r / m - r h_{t-1}),  dinitial = a g at the first position
 // The forward pass moves 4 tensors and the backward pass 7: both are bound by memory.  8 x 4096 x 5120 bf16: forward 270 us, 5.0 TB/s,
-// backward 513 us, 4.6 TB/s, where a copy of long rows reaches 6.2 and a bare pass in this pattern (tiles of 256-byte pieces of rows, 3
+// backward 503 us, 4.7 TB/s, where a copy of long rows reaches 6.2 and a bare pass in this pattern (tiles of 256-byte pieces of rows, 3
 // tensors in and 1 out, or 4 and 3) 5.1 and 5.0.  (Three vector instructions fewer per element backward left its time as it was.)
 // gated_tile.hpp says how a row is cut.  The forward pass leaves the state that enters every tile of the backward
 // pass, which then forms its own states again: one float per tile and channel instead of the states in 32 bits.
@@ -386,20 +386,20 @@ template <typename F> int with_bwd_form(Form o, F f) {
 // start of the buffer, what else it holds behind them.
 struct Plan {
   int ntiles, group, ngroups;
-  int64_t chains, steps, head;  // words of steps, bytes of tickets and words
+  int64_t chains, steps, head;  // words of steps, bytes of tickets, steps and states
   Plan(const GatedScanParams &p, Form o) {
     chains = chains_of(p);
     ntiles = (int)(tiles_of(p, o.r * o.nw) / chains);
     group = min(ntiles, chains >= 128 ? 1 : 16);
     ngroups = (ntiles + group - 1) / group;
     steps = group > 1 ? chains * ntiles * kTileChannels : 0;  // a group of one tile leaves its state alone
-    head = ntiles > 1 ? (chains * 4 + 15) / 16 * 16 + (steps + chains * ngroups * kTileChannels) * 8 : 0;
+    head = ntiles > 1 ? (chains * 4 + 15) / 16 * 16 + steps * 8 + chains * ngroups * kTileChannels * 4 : 0;
   }
   Chain chain(void *buf) const {
     Chain q;
     q.tickets = static_cast<uint32_t *>(buf);
     q.steps = reinterpret_cast<uint64_t *>(static_cast<char *>(buf) + (chains * 4 + 15) / 16 * 16);
-    q.states = q.steps + steps;
+    q.states = reinterpret_cast<uint32_t *>(q.steps + steps);
     q.ntiles = ntiles, q.group = group, q.ngroups = ngroups;
     return q;
   }

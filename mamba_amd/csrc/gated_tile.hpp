@@ -214,7 +214,8 @@ template <int V, int NW> struct WaveSteps {
 // How the tiles of one row and channel group hand the state on, always in the same order of additions.  `group` tiles
 // form a group: a tile reads the steps of the tiles before it in its group and the state at the end of the group before,
 // which that group's last tile leaves.  A word carries a step's factor and term, (bits of a, bits of b), and is written
-// in one piece: a is not negative, so its sign bit says that the word is there.  (Words are 0 before the launch.)
+// in one piece: a is not negative, so its sign bit says that the word is there.  A state's word is its bits turned by those of
+// a NaN that no state has (`kNever`), so it is not 0.  (Words are 0 before the launch.)
 // Every workgroup writes its step before it waits for others, and the workgroups of a chain take their tiles in the
 // order in which they begin (`ticket`): whatever a tile waits for has been begun and is written without waiting, or, for
 // a group's state, waits only for what lies still further ahead.  So every wait ends, in whatever order workgroups
@@ -222,7 +223,7 @@ template <int V, int NW> struct WaveSteps {
 struct Chain {
   uint32_t *tickets;  // one per chain (row and channel group)
   uint64_t *steps;    // (chain, ntiles, 64 V), none where a group is one tile
-  uint64_t *states;   // (chain, ngroups, 64 V)
+  uint32_t *states;   // (chain, ngroups, 64 V)
   int ntiles, group, ngroups;
 };
 constexpr uint64_t kThere = 1ull << 63;
@@ -235,6 +236,24 @@ DEVI float word_b(uint64_t w) { return __builtin_bit_cast(float, (uint32_t)w); }
 template <int V> DEVI void put_words(uint64_t *p, const Step<V> &s) {
 #pragma unroll
   for (int e = 0; e < V; ++e) __hip_atomic_store(p + e, word_of(s.a[e], s.b[e]), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+
+constexpr uint32_t kNever = 0x7fc00001u;
+DEVI uint32_t state_word(float h) { return (h == h ? __builtin_bit_cast(uint32_t, h) : 0x7fc00000u) ^ kNever; }
+DEVI void put_state(uint32_t *p, const Vec<2> &h) {  // both in one piece
+  __hip_atomic_store(reinterpret_cast<uint64_t *>(p), (uint64_t)state_word(h[1]) << 32 | state_word(h[0]), __ATOMIC_RELAXED,
+                     __HIP_MEMORY_SCOPE_AGENT);
+}
+// Whole wave: the states of every lane, once they are there (asked for as `wait_words` does).
+DEVI Vec<2> wait_state(const uint32_t *p) {
+  const int lane = threadIdx.x & 63;
+  const uint32_t *hint = p - lane * 2;
+  while (__hip_atomic_load(hint, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == 0) __builtin_amdgcn_s_sleep(4);
+  for (;;) {
+    const uint64_t w = __hip_atomic_load(reinterpret_cast<const uint64_t *>(p), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    if (__all(w != 0)) return Vec<2>{{__builtin_bit_cast(float, (uint32_t)w ^ kNever), __builtin_bit_cast(float, (uint32_t)(w >> 32) ^ kNever)}};
+    __builtin_amdgcn_s_sleep(1);
+  }
 }
 
 // Whole wave: the words of every lane for the tiles from p on, 64 V words apart, once those of the first `count` are there
@@ -288,12 +307,7 @@ template <int V, int NW> struct Ahead {
     }
     steps.put(wave, lane, s);
     if (wave == 0) {
-      if (g > 0) {
-        uint64_t w[1][V];
-        wait_words<V, 1>(q.states + (chain * q.ngroups + g - 1) * (64 * V) + lane * V, 1, w);
-#pragma unroll
-        for (int e = 0; e < V; ++e) first[e] = word_b(w[0][e]);
-      }
+      if (g > 0) first = wait_state(q.states + (chain * q.ngroups + g - 1) * (64 * V) + lane * V);
       state[lane] = first;
     }
   }
@@ -312,7 +326,7 @@ template <int V> DEVI void leave_step(const Chain &q, int64_t chain, int n, int 
 }
 template <int V> DEVI void leave_state(const Chain &q, int64_t chain, int n, int lane, const Vec<V> &h) {
   if (n + 1 < q.ntiles && (n + 1) % q.group == 0)
-    put_words<V>(q.states + (chain * q.ngroups + n / q.group) * (64 * V) + lane * V, Step<V>{vec_of<V>(0.f), h});
+    put_state(q.states + (chain * q.ngroups + n / q.group) * (64 * V) + lane * V, h);
 }
 
 // The tile of this workgroup within its chain: the number of workgroups of the chain that began before it.  (lds: one int.)
