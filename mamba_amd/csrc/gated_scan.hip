@@ -390,6 +390,10 @@ struct Plan {
   Plan(const GatedScanParams &p, Form o) {
     chains = chains_of(p);
     ntiles = (int)(tiles_of(p, o.r * o.nw) / chains);
+    // few chains are long ones, where states from tile to tile would be the time; many have others to run meanwhile, and a state alone
+    // is less to leave than a step and a state.  Forward + backward, us, in groups of 1 and of 16: 32 chains (32768 x 4096) 323 + 1007
+    // and 233 + 457, 64 (16384 x 8192) 221 + 595 and 224 + 448, 160 (4 x 4096 x 5120) 145 + 266 and 156 + 287, 320 (8 x) 261 + 479 and
+    // 274 + 544.  (Groups of 4: 234 + 480 at 32 chains, of 8 233 + 465, of 32 233 + 471.)
     group = min(ntiles, chains >= 128 ? 1 : 16);
     ngroups = (ntiles + group - 1) / group;
     steps = group > 1 ? chains * ntiles * kTileChannels : 0;  // a group of one tile leaves its state alone
