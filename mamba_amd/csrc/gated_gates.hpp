@@ -41,10 +41,11 @@ struct Gates {
     m2 = w < 0.25f ? near1 : else_;
   }
   DEVI float m() const { return __builtin_amdgcn_sqrtf(m2); }
-  // 1 / m, 0 where m is 0 (a gate shut to the last bit, a decay of 0): r / m tends to 0 there like sqrt(r)
+  // 1 / m, 0 where m is 0 (a gate shut to the last bit, a decay of 0): r / m tends to 0 there like sqrt(r).  Both roots take
+  // an m2 below the least normal number for 0, and the reciprocal of that is an infinity.
   DEVI float im() const {
     const float root = __builtin_amdgcn_rsqf(m2);  // (of a NaN one)
-    return m2 == 0.f ? 0.f : root;
+    return m2 < kTiny ? 0.f : root;
   }
 };
 
