@@ -6,8 +6,10 @@ namespace {
 
 // softplus to 2e-7 of its value at every size.  (An error in k repeats at every position, and a long memory adds it up;
 // softplus_f's 2e-6 near e^x = 0.05 would show in fp32 results.)  e = exp(x) with the rounding of its argument made good;
-// log(1 + e) = 2 atanh(e / (2 + e)) by its series below e = 0.5 (next term 1e-8 of the sum), the logarithm beyond.
+// log(1 + e) = 2 atanh(e / (2 + e)) by its series below e = 0.5 (next term 1e-8 of the sum), the logarithm beyond.  It is 0 in
+// 32 bits from x = -104 down; further down x log2(e) leaves their range, and its rounding is no number.
 DEVI float softplus_exact(float x) {
+  x = __builtin_elementwise_maximum(x, -200.f);  // (a NaN stays one)
   const float t = x * kLog2e, lo = __builtin_fmaf(x, kLog2e, -t) + x * 1.9259629911e-8f;  // log2(e) = kLog2e + 1.93e-8
   const float e = __builtin_amdgcn_exp2f(t) * __builtin_fmaf(lo, kLn2, 1.f);
   const float s = e * fast_rcp(2.f + e), s2 = s * s;

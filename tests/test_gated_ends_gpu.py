@@ -1,5 +1,5 @@
-"""gated_linear_scan_fn where a decay or a gate is at the end of its type's range: products of softplus and sigmoid around
-fp32's smallest normal number 2^-126."""
+"""gated_linear_scan_fn and gated_linear_state_update where a decay or a gate is at the end of its type's range: softplus of
+what lies far below zero, and products of softplus and sigmoid around fp32's smallest normal number 2^-126."""
 import pytest
 import torch
 
@@ -29,6 +29,33 @@ def _check(gate_a, decay, cu=None, dtype=torch.float32, seed=0):
     for n, v in zip(["out", "final"] + GRADS, [out, final, *grads]):
         assert torch.isfinite(v).all(), n
         within(n, v, ref[n], bound[n])
+
+
+# -2.36e38 is the least number whose product with log2(e) fp32 still holds
+FAR = [-float("inf"), -3.3e38, -2.4e38, -2.3e38, -1e30, -6e4, -1000.0, -200.0, -150.0, -1.0, 0.5]
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("L,cu", [(9, None), (150, None), (150, [0, 1, 70, 70, 149])])
+def test_decays_far_below_zero(L, cu, dtype):
+    """softplus is 0 there: the state stays what it was, and no gradient is lost to it."""
+    g = torch.Generator().manual_seed(L)
+    decay = torch.tensor([torch.finfo(dtype).min, *FAR]).to(dtype)
+    assert torch.isinf(decay).any() and not torch.isnan(decay).any()
+    _check(torch.randn(L, generator=g), decay, cu)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_step_with_decays_far_below_zero(dtype):
+    from mamba_amd.ops.gated_linear_scan import gated_linear_state_update
+    g = torch.Generator().manual_seed(0)
+    decay = torch.tensor([torch.finfo(dtype).min, *FAR]).to(dtype)
+    x, ga, gx, init = (torch.randn(3, decay.numel(), generator=g) for _ in range(4))
+    state = init.cuda()
+    out = gated_linear_state_update(state, x.cuda(), ga.cuda(), gx.cuda(), decay.cuda())
+    ref, bound = gated_linear_oracle(x[:, None], ga[:, None], gx[:, None], decay, 8.0, init)
+    within("out", out, ref["out"][:, 0], bound["out"][:, 0])
+    within("state", state, ref["final"], bound["final"])
 
 
 # k r from above 2^-126 to far below it: shut gates with ordinary decays, decays of next to nothing with open gates, and both
