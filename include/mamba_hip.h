@@ -762,7 +762,7 @@ int gated_scan_bwd(const GatedScanParams *p, mamba_stream_t stream);
 /* One position of the same recurrence: state (state_rows, dim) is updated in place, out (batch, dim) is the new state
  * in dtype.  Row state_batch_indices[b] of the state belongs to entry b (row b without them); an index outside
  * [0, state_rows) is a padding entry: no state is touched, out is 0.  The rows named have to be different ones.
- * Unit channel strides. */
+ * Unit channel strides, dim <= 2^30. */
 typedef struct GatedStepParams {
   int32_t batch, dim, state_rows;
   int32_t dtype, state_dtype, decay_dtype;

@@ -62,6 +62,7 @@ template <typename T> int step_state(const GatedStepParams &p, hipStream_t st) {
 extern "C" int gated_state_update(const GatedStepParams *p, mamba_stream_t stream) {
   if (!p || !p->state || !p->x || !p->gate_a || !p->gate_x || !p->decay || !p->out) return MAMBA_E_BADARG;
   if (p->batch <= 0 || p->dim <= 0 || p->state_rows <= 0) return MAMBA_E_BADARG;
+  if (p->dim > 1 << 30) return MAMBA_E_UNSUPPORTED;  // a lane's place in a row is counted in bytes, in 32 bits
   if (!(p->rate >= 0.f && p->rate <= 3.4e38f)) return MAMBA_E_BADARG;
   if (p->dtype < MAMBA_F32 || p->dtype > MAMBA_F16) return MAMBA_E_BADARG;
   if (!p->state_batch_indices && p->state_rows < p->batch) return MAMBA_E_BADARG;

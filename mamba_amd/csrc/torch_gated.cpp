@@ -141,7 +141,7 @@ OptTensor gated_step(const at::Tensor &state, const at::Tensor &x, const at::Ten
     if (!on_device(*t, dev) || t->scalar_type() != x.scalar_type() || t->sizes() != x.sizes() || !unit(*t)) return std::nullopt;
   const int64_t batch = x.size(0), dim = x.size(1), rows = state.size(0);
   if (!on_device(state, dev) || state.size(1) != dim || !unit(state) || !decay_ok(decay, dim, dev) || !rate_ok(rate)) return std::nullopt;
-  if (batch > INT32_MAX || dim > INT32_MAX || rows > INT32_MAX || (!indices && rows < batch) || (rows > 1 && state.stride(0) < dim))
+  if (batch > INT32_MAX || dim > (1 << 30) || rows > INT32_MAX || (!indices && rows < batch) || (rows > 1 && state.stride(0) < dim))
     return std::nullopt;
   if (indices && (!on_device(indices, dev) || indices->scalar_type() != at::kInt || indices->dim() != 1 || indices->size(0) != batch ||
                   !indices->is_contiguous()))

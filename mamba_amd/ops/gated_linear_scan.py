@@ -202,6 +202,8 @@ def gated_linear_state_update(state, x, gate_a, gate_x, decay, rate=8.0, state_b
         raise RuntimeError(f"{what}: state must be (rows, dim) and x (batch, dim)")
     batch, dim = x.shape
     _check_sizes(what, batch, dim, state.shape[0])
+    if dim > 2 ** 30:
+        raise RuntimeError(f"{what}: rows of at most 2^30 channels are served, got {dim}")
     if state_batch_indices is None and state.shape[0] < batch:
         raise RuntimeError(f"{what}: state has {state.shape[0]} rows for a batch of {batch} and no state_batch_indices")
     for name, t in (("gate_a", gate_a), ("gate_x", gate_x)):
