@@ -155,6 +155,7 @@ OptTensor gated_step(const at::Tensor &state, const at::Tensor &x, const at::Ten
   p.state_batch_indices = indices ? indices->data_ptr<int32_t>() : nullptr, p.out = out.data_ptr();
   p.state_rs = state.stride(0), p.x_rs = x.stride(0), p.gate_a_rs = ga.stride(0), p.gate_x_rs = gx.stride(0), p.out_rs = dim;
   check_rc(gated_state_update(&p, stream_of(dev)), "gated_state_update");
+  if (!state.is_inference()) state.unsafeGetTensorImpl()->bump_version();  // a graph that has saved it has to notice
   return out;
 }
 

@@ -239,6 +239,8 @@ def gated_linear_state_update(state, x, gate_a, gate_x, decay, rate=8.0, state_b
     p.state_rs, p.x_rs, p.gate_a_rs, p.gate_x_rs, p.out_rs = (t.stride(0) for t in (state, x, gate_a, gate_x, out))
     with torch.cuda.device(x.device):
         _lib.check(_lib.load().gated_state_update(p, _lib.current_stream(x.device)), "gated_state_update")
+    if not state.is_inference():
+        torch.autograd.graph.increment_version(state)  # a graph that has saved it has to notice
     return out
 
 
