@@ -131,10 +131,37 @@ pybind11::object gated_scan(const at::Tensor &x, const at::Tensor &ga, const at:
 }
 
 // ------------------------------------------------------------------ one token
+at::Tensor step(const at::Tensor &state, const at::Tensor &x, const at::Tensor &ga, const at::Tensor &gx, const at::Tensor &decay,
+                double rate, const OptTensor &indices) {
+  GatedStepParams p{};
+  p.batch = (int32_t)x.size(0), p.dim = (int32_t)x.size(1), p.state_rows = (int32_t)state.size(0);
+  p.dtype = dtype_code(x), p.state_dtype = dtype_code(state), p.decay_dtype = dtype_code(decay), p.rate = (float)rate;
+  c10::DeviceGuard guard(x.device());
+  at::Tensor out = at::empty({p.batch, p.dim}, x.options());
+  p.state = state.data_ptr(), p.x = x.data_ptr(), p.gate_a = ga.data_ptr(), p.gate_x = gx.data_ptr(), p.decay = decay.data_ptr();
+  p.state_batch_indices = indices ? indices->data_ptr<int32_t>() : nullptr, p.out = out.data_ptr();
+  p.state_rs = state.stride(0), p.x_rs = x.stride(0), p.gate_a_rs = ga.stride(0), p.gate_x_rs = gx.stride(0), p.out_rs = p.dim;
+  check_rc(gated_state_update(&p, stream_of(x.device())), "gated_state_update");
+  if (!state.is_inference()) state.unsafeGetTensorImpl()->bump_version();  // a graph that has saved it has to notice
+  return out;
+}
+
+// A call that autograd would record: there are no gradients, and a backward pass that comes to it raises.
+struct GatedStepFn : torch::autograd::Function<GatedStepFn> {
+  static at::Tensor forward(AutogradContext *, const at::Tensor &state, const at::Tensor &x, const at::Tensor &ga, const at::Tensor &gx,
+                            const at::Tensor &decay, double rate, const OptTensor &indices) {
+    return step(state, x, ga, gx, decay, rate, indices);
+  }
+  static variable_list backward(AutogradContext *, variable_list) {
+    TORCH_CHECK(false, "gated_linear_state_update has no gradients; gated_linear_scan_fn over one position has");
+    return {};
+  }
+};
+
 OptTensor gated_step(const at::Tensor &state, const at::Tensor &x, const at::Tensor &ga, const at::Tensor &gx, const at::Tensor &decay,
                      double rate, const OptTensor &indices) {
   if (!x.is_cuda() || x.dim() != 2 || state.dim() != 2 || dtype_code(x) < 0 || dtype_code(state) < 0 || x.numel() == 0 ||
-      state.size(0) == 0)
+      state.size(0) == 0 || python_call(state, x, ga, gx, decay) || records(state))
     return std::nullopt;
   const c10::Device dev = x.device();
   for (const at::Tensor *t : {&x, &ga, &gx})
@@ -146,17 +173,8 @@ OptTensor gated_step(const at::Tensor &state, const at::Tensor &x, const at::Ten
   if (indices && (!on_device(indices, dev) || indices->scalar_type() != at::kInt || indices->dim() != 1 || indices->size(0) != batch ||
                   !indices->is_contiguous()))
     return std::nullopt;
-  GatedStepParams p{};
-  p.batch = (int32_t)batch, p.dim = (int32_t)dim, p.state_rows = (int32_t)rows;
-  p.dtype = dtype_code(x), p.state_dtype = dtype_code(state), p.decay_dtype = dtype_code(decay), p.rate = (float)rate;
-  c10::DeviceGuard guard(dev);
-  at::Tensor out = at::empty({batch, dim}, x.options());
-  p.state = state.data_ptr(), p.x = x.data_ptr(), p.gate_a = ga.data_ptr(), p.gate_x = gx.data_ptr(), p.decay = decay.data_ptr();
-  p.state_batch_indices = indices ? indices->data_ptr<int32_t>() : nullptr, p.out = out.data_ptr();
-  p.state_rs = state.stride(0), p.x_rs = x.stride(0), p.gate_a_rs = ga.stride(0), p.gate_x_rs = gx.stride(0), p.out_rs = dim;
-  check_rc(gated_state_update(&p, stream_of(dev)), "gated_state_update");
-  if (!state.is_inference()) state.unsafeGetTensorImpl()->bump_version();  // a graph that has saved it has to notice
-  return out;
+  if (records(x, ga, gx, decay)) return GatedStepFn::apply(state, x, ga, gx, decay, rate, indices);
+  return step(state, x, ga, gx, decay, rate, indices);
 }
 
 // ------------------------------------------------------------------ the norm between two blocks

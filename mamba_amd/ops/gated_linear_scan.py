@@ -180,8 +180,40 @@ def gated_linear_scan_fn(x, gate_a, gate_x, decay, rate=8.0, initial_states=None
     return (out, final) if return_final_states else out
 
 
+class GatedLinearStateUpdateFn(torch.autograd.Function):
+    """Arguments as `gated_linear_state_update` has checked and converted them.  The step has no gradients: as a node it lets
+    the transforms and traces of torch see the call, and raises where a backward pass comes to it."""
+
+    @staticmethod
+    def forward(ctx, state, x, gate_a, gate_x, decay, state_batch_indices, rate):
+        batch, dim = x.shape
+        out = torch.empty(batch, dim, dtype=x.dtype, device=x.device)
+        if out.numel() == 0:
+            return out
+        if state.shape[0] == 0:  # a pool without rows: every entry is a padding entry
+            return out.zero_()
+        x, gate_a, gate_x = _unit(x), _unit(gate_a), _unit(gate_x)
+        p = _lib.GatedStepParams()
+        p.batch, p.dim, p.state_rows = batch, dim, state.shape[0]
+        p.dtype, p.state_dtype, p.decay_dtype = (_lib.DTYPE_CODE[t.dtype] for t in (x, state, decay))
+        p.rate = rate
+        p.state, p.x, p.gate_a, p.gate_x, p.decay, p.out = (t.data_ptr() for t in (state, x, gate_a, gate_x, decay, out))
+        p.state_batch_indices = _lib.ptr(state_batch_indices)
+        p.state_rs, p.x_rs, p.gate_a_rs, p.gate_x_rs, p.out_rs = (t.stride(0) for t in (state, x, gate_a, gate_x, out))
+        with torch.cuda.device(x.device):
+            _lib.check(_lib.load().gated_state_update(p, _lib.current_stream(x.device)), "gated_state_update")
+        if not state.is_inference():
+            torch.autograd.graph.increment_version(state)  # a graph that has saved it has to notice
+        return out
+
+    @staticmethod
+    def backward(ctx, dout):
+        raise RuntimeError("gated_linear_state_update has no gradients; gated_linear_scan_fn over one position has")
+
+
 def gated_linear_state_update(state, x, gate_a, gate_x, decay, rate=8.0, state_batch_indices=None):
-    """One token of the same recurrence: `state` is updated in place.
+    """One token of the same recurrence: `state` is updated in place.  It is made for generating and has no gradients: a
+    backward pass through `out` raises, and so does a call with a state that wants a gradient.
 
     Argument:
         state: (rows, dim) in fp32, fp16 or bf16, unit channel stride
@@ -220,28 +252,14 @@ def gated_linear_state_update(state, x, gate_a, gate_x, decay, rate=8.0, state_b
     if state_batch_indices is not None:
         if tuple(state_batch_indices.shape) != (batch,) or state_batch_indices.dtype not in (torch.int32, torch.int64):
             raise RuntimeError(f"{what}: state_batch_indices must be ({batch},) int32")
+    if torch.is_grad_enabled() and state.requires_grad:
+        raise RuntimeError(f"{what}: state is updated in place and takes no gradients: detach it, or call under torch.no_grad()")
     _lib.require_gpu(state, x, gate_a, gate_x, decay, state_batch_indices)
     _one_device(what, x, state, gate_a, gate_x, decay, state_batch_indices)
     if state_batch_indices is not None:
         state_batch_indices = _int32(state_batch_indices, -1, 2 ** 31 - 1)
-    out = torch.empty(batch, dim, dtype=x.dtype, device=x.device)
-    if out.numel() == 0:
-        return out
-    if state.shape[0] == 0:  # a pool without rows: every entry is a padding entry
-        return out.zero_()
-    x, gate_a, gate_x, decay = _unit(x), _unit(gate_a.to(x.dtype)), _unit(gate_x.to(x.dtype)), decay.contiguous()
-    p = _lib.GatedStepParams()
-    p.batch, p.dim, p.state_rows = batch, dim, state.shape[0]
-    p.dtype, p.state_dtype, p.decay_dtype = (_lib.DTYPE_CODE[t.dtype] for t in (x, state, decay))
-    p.rate = rate
-    p.state, p.x, p.gate_a, p.gate_x, p.decay, p.out = (t.data_ptr() for t in (state, x, gate_a, gate_x, decay, out))
-    p.state_batch_indices = _lib.ptr(state_batch_indices)
-    p.state_rs, p.x_rs, p.gate_a_rs, p.gate_x_rs, p.out_rs = (t.stride(0) for t in (state, x, gate_a, gate_x, out))
-    with torch.cuda.device(x.device):
-        _lib.check(_lib.load().gated_state_update(p, _lib.current_stream(x.device)), "gated_state_update")
-    if not state.is_inference():
-        torch.autograd.graph.increment_version(state)  # a graph that has saved it has to notice
-    return out
+    return GatedLinearStateUpdateFn.apply(state, x, gate_a.to(x.dtype), gate_x.to(x.dtype), decay.contiguous(), state_batch_indices,
+                                          rate)
 
 
 def gated_linear_state_update_ref(state, x, gate_a, gate_x, decay, rate=8.0):
