@@ -22,7 +22,8 @@ DEVI float softplus_exact(float x) {
 }
 
 // Factors of a state are positive; one that underflows is taken as the least normal number, so that an infinite state stays infinite
-// and 0 is free as a mark.  (A finite state times kTiny is gone all the same; a NaN stays one.)
+// and 0 is free as a mark.  A finite state then keeps kTiny of itself instead of nothing, and dgate_a k kTiny of it: 1e-8 where
+// they are 1e30, not worth a word below.  (A NaN stays one.)
 constexpr float kTiny = 1.17549435e-38f;
 DEVI float not_zero(float a) { return __builtin_elementwise_maximum(a, kTiny); }
 

@@ -1,6 +1,6 @@
 // One position of the gated linear recurrence (gated_scan.hip has the formulas), the states updated in place (gfx950).
 // Every operand is read once and the state and output written once: 21 MB for 256 entries of 5120 channels (bf16, fp32 states), 6.2 us
-// in a stream of calls, where a copy of that size takes 3.4; one entry of 2560 channels takes a launch, 2.6 us.  A thread has 4
+// in a stream of calls; its bytes alone are 3.4 at a large copy's rate, and one entry of 2560 channels, a launch, takes 2.6 us.  A thread has 4
 // channels of one batch entry, all its loads in flight together; many short waves fill the memory's channels.
 #include "gated_tile.hpp"
 

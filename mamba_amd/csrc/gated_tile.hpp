@@ -43,7 +43,7 @@ template <typename T, int V> struct Raw {
     for (int i = 0; i < W; ++i) w[i] = 0;
   }
   // From here on its values are formed anew: kept since they were formed first they take twice the registers of the words.  (The
-  // backward kernel spilled: 538 us at 8 x 4096 x 5120, now 512.)
+  // backward kernel of 16-bit rows spilled: 538 us at 8 x 4096 x 5120, without 512.  In 32 bits the words are the values.)
   DEVI void anew() {
     if constexpr (HALF) {
 #pragma unroll

@@ -128,7 +128,8 @@ struct Sums {
 };
 
 // Rows of more than 12 waves leave a thread 128 registers: the parameters are then read again for every row (from the
-// caches) and the next row is not asked for ahead.
+// caches) and the next row is not asked for ahead.  With a gate, LayerNorm or biases, rows of more than 8 waves (4104 channels and
+// on) spill all the same, 12 to 232 bytes a thread: 231 us at 4096 x 8192 (bf16 with gate, fp32 stream) for 118 of bytes.
 template <typename T, typename R, bool FULL, bool GATE, bool WHOLE, int MAXT>
 __global__ __launch_bounds__(MAXT) void norm_block_bwd_kernel(const NormBlockParams p, const Sums sums) {
   __shared__ float lds[64];
@@ -238,7 +239,9 @@ __global__ __launch_bounds__(MAXT) void norm_block_bwd_kernel(const NormBlockPar
 }
 
 // ------------------------------------------------------------------ any row
-// One row of any length, read again from memory for every pass over it: rows of less than 8 or more than 8192 channels.
+// One row of any length, read again from memory for every pass over it: rows of less than 8 or more than 8192 channels.  The long
+// ones are served, not made fast: 283 us forward and 941 backward at 4096 x 8198 (bf16 with gate, fp32 stream), where 8192 channels in
+// registers take 88 and 231.
 constexpr int kThreads = 256;
 
 DEVI float block_sum(float v, float *red) {

@@ -5,7 +5,8 @@
     r_t = sigmoid(gate_a_t),  i_t = sigmoid(gate_x_t),  log a_t = -rate * softplus(decay) * r_t
     h_t = a_t * h_{t-1} + sqrt(1 - a_t^2) * i_t * x_t
 
-per channel.  The states, the decays and every sum are held in fp32.  There is no CPU or PyTorch fallback: CPU tensors
+per channel.  The first position of a sequence is like any other: what enters there is scaled by sqrt(1 - a_t^2) too (there is no
+form with the factor 1 in its place).  The states, the decays and every sum are held in fp32.  There is no CPU or PyTorch fallback: CPU tensors
 raise.  `gated_linear_scan_ref` and `gated_linear_state_update_ref` state the arithmetic in plain torch; no operator
 calls them.
 """
