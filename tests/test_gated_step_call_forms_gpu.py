@@ -62,6 +62,11 @@ def test_a_state_of_inference_mode(host):
         state = t["state"].clone()
     with torch.no_grad():
         assert torch.equal(_step(state, **{n: t[n] for n in NAMES[1:]}), want)
+    with torch.inference_mode():
+        state = t["state"].clone()
+        rest = {n: t[n].clone() for n in NAMES[1:4]}
+    t["decay"].requires_grad_()  # a call that autograd records
+    assert torch.equal(_step(state, **rest, decay=t["decay"]), want)
 
 
 @pytest.mark.parametrize("which", NAMES)
