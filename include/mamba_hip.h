@@ -823,6 +823,102 @@ int norm_block_fwd(const NormBlockParams *p, mamba_stream_t stream);
 int norm_block_bwd(const NormBlockParams *p, mamba_stream_t stream);
 int norm_block_bwd_nparts(const NormBlockParams *p);
 
+/* -------------------------------------------------------------------------
+ * Linear attention with a decay per head, over rows of a batch or over packed sequences:
+ *   S_t = exp(log_decay[h]) S_{t-1} + k_t v_t^T   (headdim_k x headdim_v),   out_t = scale q_t S_t
+ * q, out, dout, dq are (batch, seqlen, nheads, headdim_k or _v) of `dtype`, k, v, dk, dv (batch, seqlen, nkvheads, ..): nheads /
+ * nkvheads neighbouring heads share keys and values.  Unit stride along the head, batch, position and head strides given (any
+ * alignment).  log_decay (nheads) fp32: minus infinity is a decay to nothing, values above 0 count as 0.  States are dense fp32:
+ * (batch or nseq, nheads, headdim_k, headdim_v).
+ * cu_seqlens (nseq + 1 int32, batch 1, not decreasing) packs nseq sequences into the row: sequence q has the positions
+ * cu_seqlens[q] .. cu_seqlens[q + 1] - 1 and starts from its own initial state.  Positions before the first and behind the last
+ * sequence count for nothing: their outputs and gradients are 0.
+ * Head sizes up to 256, seqlen up to 2^30.  ws: linear_attn_fwd_ws_bytes / linear_attn_bwd_ws_bytes of 16-byte aligned memory
+ * (0: none), contents ignored on entry, nothing in it is kept between calls.  Every result repeats bit for bit.
+ * ------------------------------------------------------------------------- */
+typedef struct LinearAttnParams {
+  int32_t batch, seqlen, nheads, nkvheads, headdim_k, headdim_v;
+  int32_t nseq; /* 0: the rows of the batch are the sequences */
+  int32_t dtype;
+  float scale;
+  int32_t reserved;
+  const void *q, *k, *v;
+  const float *log_decay;
+  const float *initial_states; /* nullable: zeros */
+  const int32_t *cu_seqlens;   /* null iff nseq is 0 */
+  void *out;                   /* forward only */
+  float *final_states;         /* forward only, nullable */
+  void *ws;
+  int64_t q_bs, q_ls, q_hs, k_bs, k_ls, k_hs, v_bs, v_ls, v_hs, out_bs, out_ls, out_hs;
+  /* ---- backward only ---- */
+  const void *dout;
+  const float *dfinal_states; /* nullable */
+  void *dq, *dk, *dv;
+  float *dinitial_states; /* nullable */
+  int64_t dout_bs, dout_ls, dout_hs, dq_bs, dq_ls, dq_hs, dk_bs, dk_ls, dk_hs, dv_bs, dv_ls, dv_hs;
+} LinearAttnParams;
+
+int64_t linear_attn_fwd_ws_bytes(const LinearAttnParams *p);
+int64_t linear_attn_bwd_ws_bytes(const LinearAttnParams *p);
+int linear_attn_fwd(const LinearAttnParams *p, mamba_stream_t stream);
+int linear_attn_bwd(const LinearAttnParams *p, mamba_stream_t stream);
+
+/* One position of the same recurrence: state (state_rows, nheads, headdim_k, headdim_v), each row dense, is updated in place,
+ * out (batch, nheads, headdim_v) is scale q S of the new state.  Row state_batch_indices[b] of the state belongs to entry b (row b
+ * without them); an index outside [0, state_rows) is a padding entry: no state is touched, out is 0.  The rows named have to be
+ * different ones.  Up to 65535 heads. */
+typedef struct LinearAttnStepParams {
+  int32_t batch, nheads, nkvheads, headdim_k, headdim_v, state_rows;
+  int32_t dtype, state_dtype;
+  float scale;
+  int32_t reserved;
+  void *state;
+  const void *q, *k, *v;
+  const float *log_decay;
+  const int32_t *state_batch_indices; /* nullable */
+  void *out;
+  int64_t state_rs, q_bs, q_hs, k_bs, k_hs, v_bs, v_hs, out_bs, out_hs;
+} LinearAttnStepParams;
+
+int linear_attn_state_update(const LinearAttnStepParams *p, mamba_stream_t stream);
+
+/* -------------------------------------------------------------------------
+ * Attention of one new token per sequence over a paged cache of keys and values:
+ *   out[b, h] = sum_p softmax_p(scale q[b, h] . K[p, h / group]) V[p, h / group],   group = nheads / nkvheads
+ * Position p of sequence b lies in page block_table[b, p / page_size] at p % page_size: k_cache (num_pages, page_size, nkvheads,
+ * headdim_k), v_cache (.., headdim_v), unit stride along the head, the other strides given.  cache_seqlens[b] positions are in the
+ * cache.  With k and v (the new token's, both or neither) the token is position cache_seqlens[b]: it is written there and takes
+ * part; without, the cache is only read.  window > 0: only the last `window` positions, the new one among them.
+ * A negative cache_seqlens[b] is a padding entry: nothing is written, out is 0; so it is where no position counts.  A length
+ * beyond max_pages * page_size counts as that.  Pages outside of [0, num_pages) have no positions: they are left out, and a token
+ * whose page is one takes part without being written.
+ * nsplit parts of the cache's length are worked on side by side (paged_attn_parts says how many suit; 1: no workspace);
+ * ws: paged_attn_ws_bytes of 16-byte aligned memory, contents ignored on entry.  Head sizes up to 256, max_pages * page_size up to
+ * 2^30, batch up to 65535.
+ * ------------------------------------------------------------------------- */
+typedef struct PagedAttnParams {
+  int32_t batch, nheads, nkvheads, headdim_k, headdim_v;
+  int32_t num_pages, page_size, max_pages;
+  int32_t window; /* 0: all positions */
+  int32_t nsplit;
+  int32_t dtype;
+  float scale;
+  const void *q;
+  const void *k, *v; /* nullable */
+  void *k_cache, *v_cache;
+  const int32_t *block_table;
+  const int32_t *cache_seqlens;
+  void *out;
+  float *ws;
+  int64_t q_bs, q_hs, k_bs, k_hs, v_bs, v_hs, out_bs, out_hs;
+  int64_t kc_ps, kc_ls, kc_hs, vc_ps, vc_ls, vc_hs; /* page, position, head */
+  int64_t table_bs;
+} PagedAttnParams;
+
+int paged_attn_parts(const PagedAttnParams *p);
+int64_t paged_attn_ws_bytes(const PagedAttnParams *p);
+int paged_attn_update(const PagedAttnParams *p, mamba_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -171,6 +171,41 @@ class NormBlockParams(ctypes.Structure):
     )
 
 
+def _strides(*names):
+    return [(f"{n}_{d}", c_i64) for n in names for d in ("bs", "ls", "hs")]
+
+
+class LinearAttnParams(ctypes.Structure):
+    _fields_ = (
+        [(n, c_i32) for n in ("batch", "seqlen", "nheads", "nkvheads", "headdim_k", "headdim_v", "nseq", "dtype")]
+        + [("scale", c_f32), ("reserved", c_i32)]
+        + [(n, c_vp) for n in ("q", "k", "v", "log_decay", "initial_states", "cu_seqlens", "out", "final_states", "ws")]
+        + _strides("q", "k", "v", "out")
+        + [(n, c_vp) for n in ("dout", "dfinal_states", "dq", "dk", "dv", "dinitial_states")]
+        + _strides("dout", "dq", "dk", "dv")
+    )
+
+
+class LinearAttnStepParams(ctypes.Structure):
+    _fields_ = (
+        [(n, c_i32) for n in ("batch", "nheads", "nkvheads", "headdim_k", "headdim_v", "state_rows", "dtype", "state_dtype")]
+        + [("scale", c_f32), ("reserved", c_i32)]
+        + [(n, c_vp) for n in ("state", "q", "k", "v", "log_decay", "state_batch_indices", "out")]
+        + [(n, c_i64) for n in ("state_rs", "q_bs", "q_hs", "k_bs", "k_hs", "v_bs", "v_hs", "out_bs", "out_hs")]
+    )
+
+
+class PagedAttnParams(ctypes.Structure):
+    _fields_ = (
+        [(n, c_i32) for n in ("batch", "nheads", "nkvheads", "headdim_k", "headdim_v", "num_pages", "page_size", "max_pages", "window",
+                              "nsplit", "dtype")]
+        + [("scale", c_f32)]
+        + [(n, c_vp) for n in ("q", "k", "v", "k_cache", "v_cache", "block_table", "cache_seqlens", "out", "ws")]
+        + [(n, c_i64) for n in ("q_bs", "q_hs", "k_bs", "k_hs", "v_bs", "v_hs", "out_bs", "out_hs", "kc_ps", "kc_ls", "kc_hs", "vc_ps",
+                                "vc_ls", "vc_hs", "table_bs")]
+    )
+
+
 _lib = None
 
 
@@ -268,6 +303,18 @@ def load():
     for name in ("gated_scan_ckpt_bytes", "gated_scan_bwd_ws_bytes"):
         fn = getattr(lib, name)
         fn.argtypes = [ctypes.POINTER(GatedScanParams)]
+        fn.restype = c_i64
+    for name, params in (("linear_attn_fwd", LinearAttnParams), ("linear_attn_bwd", LinearAttnParams),
+                         ("linear_attn_state_update", LinearAttnStepParams), ("paged_attn_update", PagedAttnParams)):
+        fn = getattr(lib, name)
+        fn.argtypes = [ctypes.POINTER(params), c_vp]
+        fn.restype = ctypes.c_int
+    lib.paged_attn_parts.argtypes = [ctypes.POINTER(PagedAttnParams)]
+    lib.paged_attn_parts.restype = ctypes.c_int
+    for name, params in (("linear_attn_fwd_ws_bytes", LinearAttnParams), ("linear_attn_bwd_ws_bytes", LinearAttnParams),
+                         ("paged_attn_ws_bytes", PagedAttnParams)):
+        fn = getattr(lib, name)
+        fn.argtypes = [ctypes.POINTER(params)]
         fn.restype = c_i64
     for name in ("norm_residual_fwd", "norm_residual_bwd"):
         fn = getattr(lib, name)

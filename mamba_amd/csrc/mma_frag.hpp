@@ -1,0 +1,160 @@
+// Operand fragments of the 16 x 16 matrix instructions for kernels whose products feed one another in registers (linear
+// attention, attention over a cache), for the three types of operands.
+//
+// D = A B^T per tile: lane (i = lane % 16, g = lane / 16) supplies row i of A and of B at the k values of its group and
+// holds D[m][n] at n = i, m = 4 g + r.  So a lane that holds a result for one n and 4 consecutive m holds, read as an
+// operand, row n at 4 consecutive k: results become operands where they lie.  A fragment spans KS values of k, NT = KS / 16
+// tiles of results make one, and `krow` says which of the KS rows of a block the tile `half` has to take for that.
+//   bf16: one instruction for 32 k.  fp16: data times data as it is (exact); where one side has been computed (a weighted
+//   sum leaves fp16's range at 65504) both sides are split into two bf16 parts, 16 bits together, three instructions.
+//   fp32: four instructions of 4 k, products and sums in fp32.
+// Data: fragments that hold operands as they lie in memory.  Wide: a computed one in two parts.  Comp: a computed one in as
+// many parts as the result's type can show.
+#pragma once
+#include "common.hpp"
+
+typedef __bf16 frag_bf16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 frag_f16x8 __attribute__((ext_vector_type(8)));
+typedef short frag_i16x4 __attribute__((ext_vector_type(4)));
+typedef short frag_i16x8 __attribute__((ext_vector_type(8)));
+
+DEVI f32x4 mma16(frag_bf16x8 a, frag_bf16x8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
+DEVI f32x4 mma16(frag_f16x8 a, frag_f16x8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
+
+// two bf16 parts of eight values: 8 + 8 bits
+struct Split {
+  frag_bf16x8 h, l;
+  DEVI void set(const float (&v)[8]) {
+    u32x4 hi, lo;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      hi[e] = pack_bf16(v[2 * e], v[2 * e + 1]);
+      lo[e] = pack_bf16(v[2 * e] - bf16_lo(hi[e]), v[2 * e + 1] - bf16_hi(hi[e]));
+    }
+    h = __builtin_bit_cast(frag_bf16x8, hi);
+    l = __builtin_bit_cast(frag_bf16x8, lo);
+  }
+};
+DEVI f32x4 mma16(const Split &a, const Split &b, f32x4 c) { return mma16(a.h, b.h, mma16(a.h, b.l, mma16(a.l, b.h, c))); }
+DEVI f32x4 mma16(const Split &a, frag_bf16x8 b, f32x4 c) { return mma16(a.h, b, mma16(a.l, b, c)); }
+DEVI f32x4 mma16(frag_bf16x8 a, const Split &b, f32x4 c) { return mma16(a, b.h, mma16(a, b.l, c)); }
+
+struct Frag32 {
+  f32x4 v;
+};
+DEVI f32x4 mma16(const Frag32 &a, const Frag32 &b, f32x4 c) {
+#pragma unroll
+  for (int r = 0; r < 4; ++r) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a.v[r], b.v[r], c, 0, 0, 0);
+  return c;
+}
+
+// 4 rows x 16 columns of 16-bit values, the hardware hands lane i column i of the rows: `src` is this lane's piece of 4 columns
+// of row i / 4.
+DEVI frag_i16x4 lds_transposed(const uint16_t *src) {
+  typedef __attribute__((address_space(3))) frag_i16x4 *lds_ptr;
+  return __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)src);
+}
+
+template <typename T> struct Frags16 {
+  using E = uint16_t;  // as it lies in LDS
+  static constexpr int KS = 32, NT = 2, V = 8, PAD = 8;
+  static DEVI int krow(int m, int half) { return 8 * (m >> 2) + (m & 3) + 4 * half; }
+  // row i of a tile whose rows lie along k: k .. k + 7 from `at` (16-byte aligned)
+  static DEVI u32x4 along(const E *at) { return *reinterpret_cast<const u32x4 *>(at); }
+  // A block of KS rows of pitch P that lie along k: lane i gets column `i` of the 16 whose pieces of 4 lie at
+  // `first + step * (i % 4)` of a row.
+  template <int P> static DEVI u32x4 across(const E *block, int first, int step, int i, int g) {
+    const E *src = block + (8 * g + (i >> 2)) * P + first + step * (i & 3);
+    const frag_i16x4 lo = lds_transposed(src), hi = lds_transposed(src + 4 * P);
+    return __builtin_bit_cast(u32x4, (frag_i16x8)__builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+  }
+  // the 16 columns of tile `half` of a block of 32: in the order of krow, or one after the other
+  template <int P> static DEVI u32x4 columns(const E *block, int col, int half, int i, int g) {
+    return across<P>(block, col + 4 * half, 8, i, g);
+  }
+  template <int P> static DEVI u32x4 columns_in_order(const E *block, int col, int i, int g) { return across<P>(block, col, 4, i, g); }
+  static DEVI void gather(const f32x4 (&t)[2], float (&v)[8]) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] = t[0][e], v[4 + e] = t[1][e];
+  }
+};
+
+template <typename T> struct Frags;
+template <> struct Frags<bf16_t> : Frags16<bf16_t> {
+  using Raw = u32x4;
+  using Data = frag_bf16x8;
+  using Comp = frag_bf16x8;
+  using Wide = Split;
+  static DEVI Data data(u32x4 w) { return __builtin_bit_cast(frag_bf16x8, w); }
+  static DEVI f32x4 mma_raw(u32x4 a, u32x4 b, f32x4 c) { return mma16(data(a), data(b), c); }
+  static DEVI void unpack(u32x4 w, float (&v)[8]) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[2 * e] = bf16_lo(w[e]), v[2 * e + 1] = bf16_hi(w[e]);
+  }
+  static DEVI u32x4 pack(const float (&v)[8]) {
+    return u32x4{pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3]), pack_bf16(v[4], v[5]), pack_bf16(v[6], v[7])};
+  }
+  static DEVI Comp comp(const float (&v)[8]) { return data(pack(v)); }
+  static DEVI Wide wide(const float (&v)[8]) {
+    Split s;
+    s.set(v);
+    return s;
+  }
+};
+template <> struct Frags<f16_t> : Frags16<f16_t> {
+  using Raw = u32x4;
+  using Data = Split;
+  using Comp = Split;
+  using Wide = Split;
+  static DEVI void unpack(u32x4 w, float (&v)[8]) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[2 * e] = f16_lo(w[e]), v[2 * e + 1] = f16_hi(w[e]);
+  }
+  static DEVI u32x4 pack(const float (&v)[8]) {
+    return u32x4{pack_f16(v[0], v[1]), pack_f16(v[2], v[3]), pack_f16(v[4], v[5]), pack_f16(v[6], v[7])};
+  }
+  static DEVI Data data(u32x4 w) {
+    float v[8];
+    unpack(w, v);
+    return wide(v);
+  }
+  static DEVI f32x4 mma_raw(u32x4 a, u32x4 b, f32x4 c) {
+    return mma16(__builtin_bit_cast(frag_f16x8, a), __builtin_bit_cast(frag_f16x8, b), c);
+  }
+  static DEVI Split wide(const float (&v)[8]) {
+    Split s;
+    s.set(v);
+    return s;
+  }
+  static DEVI Comp comp(const float (&v)[8]) { return wide(v); }
+};
+template <> struct Frags<float> {
+  using E = float;
+  using Raw = f32x4;
+  using Data = Frag32;
+  using Comp = Frag32;
+  using Wide = Frag32;
+  static constexpr int KS = 16, NT = 1, V = 4, PAD = 4;
+  static DEVI int krow(int m, int) { return m; }
+  static DEVI f32x4 along(const E *at) { return *reinterpret_cast<const f32x4 *>(at); }
+  template <int P> static DEVI f32x4 columns_in_order(const E *block, int col, int i, int g) {
+    f32x4 v;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) v[r] = block[(4 * g + r) * P + col + i];
+    return v;
+  }
+  template <int P> static DEVI f32x4 columns(const E *block, int col, int, int i, int g) { return columns_in_order<P>(block, col, i, g); }
+  static DEVI void gather(const f32x4 (&t)[1], float (&v)[4]) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] = t[0][e];
+  }
+  static DEVI Data data(f32x4 w) { return Frag32{w}; }
+  static DEVI f32x4 mma_raw(f32x4 a, f32x4 b, f32x4 c) { return mma16(Frag32{a}, Frag32{b}, c); }
+  static DEVI void unpack(f32x4 w, float (&v)[4]) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] = w[e];
+  }
+  static DEVI f32x4 pack(const float (&v)[4]) { return f32x4{v[0], v[1], v[2], v[3]}; }
+  static DEVI Frag32 comp(const float (&v)[4]) { return Frag32{f32x4{v[0], v[1], v[2], v[3]}}; }
+  static DEVI Frag32 wide(const float (&v)[4]) { return comp(v); }
+};

@@ -1,0 +1,333 @@
+// Attention of one new token over a paged cache of keys and values, split over the cache's length and joined (gfx950):
+//   out = sum_p softmax_p(scale q . k_p) v_p   over the positions of the sequence's cache (the last `window` of them)
+// Every key and value is read once, for all query heads that share it: that is what the operator costs (16 operations a byte for
+// 16 heads).  A workgroup has one key head (up to 16 of its query heads) and a run of positions; each of its waves takes a tile of
+// 32 positions (fp32: 16) at a time and keeps the running maximum m and the sums
+//   l = sum 2^(s_p - m),  o = sum 2^(s_p - m) v_p,   s_p = scale log2(e) q . k_p
+// As the rows of K sit in memory they are operands; the products leave the tile with 8 positions of one head in a lane, which is
+// the operand that the product with V wants (mma_frag.hpp), and a head's m, l are one lane's; V goes through LDS to be read by
+// columns.  Waves meet at the end, workgroups in a second launch.
+#include "mma_frag.hpp"
+
+#include <algorithm>
+#include <type_traits>
+
+namespace {
+
+constexpr int kThreads = 256, kWaves = 4, kHeads = 16;
+constexpr float kLow = -3e38f;  // stands for a maximum of minus infinity, so that differences are numbers
+
+struct Span {  // positions of a sequence, in tiles
+  int n;         // positions of the cache before the call; -1: an empty place of the batch
+  int first, last;  // [first, last): those that count
+  int tile0, tiles; // tiles that hold them
+  int per, parts;   // tiles of a part, parts that have any
+};
+// At least two tiles a wave and part, so that short sequences are not cut for the sake of long ones.
+template <int KS> DEVI Span span_of(const PagedAttnParams &p, int b) {
+  Span r;
+  r.n = min(p.cache_seqlens[b], p.max_pages * p.page_size);
+  r.last = max(r.n, -1) + (p.k ? 1 : 0);
+  r.first = p.window > 0 ? max(r.last - p.window, 0) : 0;
+  r.tile0 = r.first / KS;
+  r.tiles = r.last > r.first ? (r.last - 1) / KS + 1 - r.tile0 : 0;
+  r.per = max((r.tiles + p.nsplit - 1) / p.nsplit, 2 * kWaves);
+  r.parts = (r.tiles + r.per - 1) / r.per;
+  return r;
+}
+
+// ws: per (batch, head, part) D sums o, then per (batch, head, part) m and l
+template <int D> DEVI int64_t part_at(const PagedAttnParams &p, int b, int h, int part) {
+  return ((int64_t)b * p.nheads + h) * p.nsplit + part;
+}
+
+template <typename T, int D, bool RAG> __global__ __launch_bounds__(kThreads) void paged_part_kernel(const PagedAttnParams p) {
+  using F = Frags<T>;
+  using E = typename F::E;
+  using Raw = typename F::Raw;
+  constexpr int KS = F::KS, NT = F::NT, V = F::V, KB = D / KS, OT = D / 16, PER = D / V, NV = KS * PER / 64, PITCH = D + F::PAD;
+  constexpr int AREA = KS * PITCH * (int)sizeof(E) > kHeads * (D + 4) * 4 ? KS * PITCH * (int)sizeof(E) : kHeads * (D + 4) * 4;
+  __shared__ __align__(16) char area[kWaves][AREA];
+  __shared__ float wave_m[kWaves][kHeads], wave_l[kWaves][kHeads];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), i = lane & 15, g = lane >> 4;
+  const int group = p.nheads / p.nkvheads, htiles = (group + kHeads - 1) / kHeads;
+  const int part = blockIdx.x, hk = blockIdx.y / htiles, ht = blockIdx.y % htiles, b = blockIdx.z;
+  const int h0 = hk * group + ht * kHeads, heads = min(group - ht * kHeads, kHeads);
+  const Span sp = span_of<KS>(p, b);
+  if (part > 0 && part >= sp.parts) return;
+  const int begin = sp.tile0 + part * sp.per, end = min(begin + sp.per, sp.tile0 + sp.tiles);
+  const int dk = p.headdim_k, dv = p.headdim_v;
+  const int32_t *table = p.block_table + b * p.table_bs;
+  const T *k_new = p.k ? static_cast<const T *>(p.k) + b * p.k_bs + hk * p.k_hs : nullptr;
+  const T *v_new = p.k ? static_cast<const T *>(p.v) + b * p.v_bs + hk * p.v_hs : nullptr;
+
+  // the new token's row of the cache: written here, read by nobody (its tile takes the row from the call's arguments)
+  if (k_new && ht == 0 && part == max(sp.parts - 1, 0) && sp.n >= 0 && sp.n < p.max_pages * p.page_size) {
+    const int id = table[sp.n / p.page_size], off = sp.n % p.page_size;
+    if (id >= 0 && id < p.num_pages) {
+      T *kd = static_cast<T *>(p.k_cache) + id * p.kc_ps + off * p.kc_ls + hk * p.kc_hs;
+      T *vd = static_cast<T *>(p.v_cache) + id * p.vc_ps + off * p.vc_ls + hk * p.vc_hs;
+      for (int x = tid; x < dk; x += kThreads) kd[x] = k_new[x];
+      for (int x = tid; x < dv; x += kThreads) vd[x] = v_new[x];
+    }
+  }
+
+  // q of the heads, by lanes: head i (beyond the last: the last again, not stored)
+  Raw qf[KB];
+  const T *q = static_cast<const T *>(p.q) + b * p.q_bs + (h0 + min(i, heads - 1)) * p.q_hs;
+  auto piece = [&](const T *row, int col, int cols) -> Raw {  // columns from `cols` on become 0
+    if constexpr (RAG) {
+      E v[V];
+#pragma unroll
+      for (int e = 0; e < V; ++e) v[e] = *(const GLOBAL_AS E *)(row + min(col + e, cols - 1));
+#pragma unroll
+      for (int e = 0; e < V; ++e) v[e] = col + e < cols ? v[e] : E(0);
+      return __builtin_bit_cast(Raw, v);
+    } else {
+      Raw v;
+      const T *at = row + min(col, cols - V);
+      if constexpr (std::is_same_v<T, float>) v = *(const GLOBAL_AS f32x4_a4 *)at;
+      else v = *(const GLOBAL_AS u32x4_a2 *)at;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[e] = col < cols ? v[e] : 0;
+      return v;
+    }
+  };
+#pragma unroll
+  for (int kb = 0; kb < KB; ++kb) qf[kb] = piece(q, KS * kb + V * g, dk);
+
+  // rows of a tile: lane r (of KS) has the place of position r; those that do not count take the first one's that does
+  auto page_of = [&](int tile) {
+    const int pos = KS * tile + (lane & (KS - 1));
+    return table[min(pos / p.page_size, p.max_pages - 1)];
+  };
+  struct Rows {
+    uint64_t k, v;
+    uint32_t mask;
+  };
+  auto rows_of = [&](int tile, int id) {
+    const int pos = KS * tile + (lane & (KS - 1)), off = pos % p.page_size;
+    const bool is_new = k_new && pos == sp.n;
+    const bool ok = pos >= sp.first && pos < sp.last && (is_new || (id >= 0 && id < p.num_pages && pos / p.page_size < p.max_pages));
+    const int64_t page = min(max(id, 0), p.num_pages - 1);
+    const T *kr = static_cast<const T *>(p.k_cache) + page * p.kc_ps + off * p.kc_ls + hk * p.kc_hs;
+    const T *vr = static_cast<const T *>(p.v_cache) + page * p.vc_ps + off * p.vc_ls + hk * p.vc_hs;
+    Rows r;
+    r.k = reinterpret_cast<uint64_t>(is_new ? k_new : kr), r.v = reinterpret_cast<uint64_t>(is_new ? v_new : vr);
+    r.mask = (uint32_t)__ballot(ok) & (uint32_t)((1ull << KS) - 1);
+    const int src = ok || !r.mask ? (lane & (KS - 1)) : __builtin_ctz(r.mask);
+    r.k = __shfl(r.k, src, 64), r.v = __shfl(r.v, src, 64);
+    return r;
+  };
+  Raw kr[KB][NT], vr[NV];
+  auto load_k = [&](const Rows &r) {
+#pragma unroll
+    for (int h = 0; h < NT; ++h) {
+      const T *row = reinterpret_cast<const T *>(__shfl(r.k, F::krow(i, h), 64));
+#pragma unroll
+      for (int kb = 0; kb < KB; ++kb) kr[kb][h] = piece(row, KS * kb + V * g, dk);
+    }
+  };
+  auto load_v = [&](const Rows &r) {
+#pragma unroll
+    for (int n = 0; n < NV; ++n) {
+      const int id = n * 64 + lane;
+      vr[n] = piece(reinterpret_cast<const T *>(__shfl(r.v, id / PER, 64)), id % PER * V, dv);
+    }
+  };
+
+  E *tile_v = reinterpret_cast<E *>(area[wave]);
+  const float scale = p.scale * kLog2e;
+  float m = -__builtin_inff(), l = 0.f;
+  f32x4 o[OT];
+#pragma unroll
+  for (int d = 0; d < OT; ++d) o[d] = f32x4{0.f, 0.f, 0.f, 0.f};
+
+  int t = begin + wave;
+  Rows now{}, next{};
+  int id_next = 0;
+  if (t < end) {
+    now = rows_of(t, page_of(t));
+    load_k(now), load_v(now);
+    if (t + kWaves < end) id_next = page_of(t + kWaves);
+  }
+  for (; t < end; t += kWaves) {
+    const bool more = t + kWaves < end;
+    f32x4 s[NT];
+#pragma unroll
+    for (int h = 0; h < NT; ++h) {
+      s[h] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int kb = 0; kb < KB; ++kb) s[h] = F::mma_raw(kr[kb][h], qf[kb], s[h]);
+    }
+    if (more) {
+      next = rows_of(t + kWaves, id_next);
+      load_k(next);
+      if (t + 2 * kWaves < end) id_next = page_of(t + 2 * kWaves);
+    }
+#pragma unroll
+    for (int n = 0; n < NV; ++n) {
+      const int id = n * 64 + lane;
+      *reinterpret_cast<Raw *>(tile_v + id / PER * PITCH + id % PER * V) = vr[n];
+    }
+    if (more) load_v(next);
+    if (now.mask) {
+      float v[V];
+      F::gather(s, v);
+      const uint32_t mine = now.mask >> (V * g);
+      float top = -__builtin_inff();
+#pragma unroll
+      for (int e = 0; e < V; ++e) {
+        v[e] = (mine >> e & 1) ? v[e] * scale : -__builtin_inff();
+        top = fmaxf(top, v[e]);
+      }
+      top = fmaxf(top, __shfl_xor(top, 16, 64));
+      top = fmaxf(top, __shfl_xor(top, 32, 64));
+      const float m_new = fmaxf(fmaxf(m, top), kLow), shrink = fast_exp2(m - m_new);
+      m = m_new;
+      l *= shrink;
+#pragma unroll
+      for (int e = 0; e < V; ++e) {
+        v[e] = fast_exp2(v[e] - m);
+        l += v[e];
+      }
+      const Raw pf = F::pack(v);  // 0 .. 1: the type's own format holds them; l has them unrounded
+#pragma unroll
+      for (int d = 0; d < OT; ++d) {
+        o[d] *= shrink;
+        o[d] = F::mma_raw(F::template columns_in_order<PITCH>(tile_v, 16 * d, i, g), pf, o[d]);
+      }
+    }
+    now = next;
+  }
+
+  // the waves' shares together: lane (i, g) has head i, values 16 d + 4 g ..; l is the sum over a head's four lanes
+  l += __shfl_xor(l, 16, 64);
+  l += __shfl_xor(l, 32, 64);
+  asm volatile("" ::: "memory");  // the same LDS as numbers of another type
+  float *mine = reinterpret_cast<float *>(area[wave]) + i * (D + 4);
+#pragma unroll
+  for (int d = 0; d < OT; ++d) *reinterpret_cast<f32x4 *>(mine + 16 * d + 4 * g) = o[d];
+  if (g == 0) wave_m[wave][i] = m, wave_l[wave][i] = l;
+  __syncthreads();
+  for (int x = tid; x < heads * D; x += kThreads) {
+    const int h = x / D, col = x % D;
+    float top = -__builtin_inff(), sum = 0.f, acc = 0.f;
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) top = fmaxf(top, wave_m[w][h]);
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) {
+      if (wave_m[w][h] == -__builtin_inff()) continue;  // a wave that has seen no position
+      const float f = fast_exp2(wave_m[w][h] - top);
+      sum = __builtin_fmaf(f, wave_l[w][h], sum);
+      acc = __builtin_fmaf(f, reinterpret_cast<const float *>(area[w])[h * (D + 4) + col], acc);
+    }
+    const bool none = top == -__builtin_inff();
+    if (p.nsplit == 1 || sp.parts <= 1) {
+      if (col < dv) st1<T>(static_cast<T *>(p.out) + b * p.out_bs + (h0 + h) * p.out_hs + col, none ? 0.f : acc / sum);
+    } else {
+      const int64_t at = part_at<D>(p, b, h0 + h, part);
+      p.ws[at * D + col] = acc;
+      if (col == 0) {
+        float *ml = p.ws + (int64_t)p.batch * p.nheads * p.nsplit * D + at * 2;
+        ml[0] = top, ml[1] = sum;
+      }
+    }
+  }
+}
+
+// The parts of a sequence together: one workgroup per (batch, head), its waves take parts in turn.
+template <typename T, int D, int KS> __global__ __launch_bounds__(kThreads) void paged_join_kernel(const PagedAttnParams p) {
+  constexpr int TURN = kThreads / D;
+  __shared__ float acc_of[TURN][D], sum_of[TURN];
+  const int h = blockIdx.x, b = blockIdx.y;
+  const Span sp = span_of<KS>(p, b);
+  if (sp.parts <= 1) return;
+  const int col = threadIdx.x % D, turn = threadIdx.x / D;
+  const int64_t at0 = part_at<D>(p, b, h, 0);
+  const float *ml = p.ws + (int64_t)p.batch * p.nheads * p.nsplit * D + at0 * 2;
+  float top = -__builtin_inff();
+  for (int s = 0; s < sp.parts; ++s) top = fmaxf(top, ml[2 * s]);
+  float sum = 0.f, acc = 0.f;
+  for (int s = turn; s < sp.parts; s += TURN) {
+    if (ml[2 * s] == -__builtin_inff()) continue;
+    const float f = fast_exp2(ml[2 * s] - top);
+    sum = __builtin_fmaf(f, ml[2 * s + 1], sum);
+    acc = __builtin_fmaf(f, p.ws[(at0 + s) * D + col], acc);
+  }
+  acc_of[turn][col] = acc;
+  if (col == 0) sum_of[turn] = sum;
+  __syncthreads();
+  if (turn == 0 && col < p.headdim_v) {
+    sum = 0.f, acc = 0.f;
+#pragma unroll
+    for (int t = 0; t < TURN; ++t) sum += sum_of[t], acc += acc_of[t][col];
+    st1<T>(static_cast<T *>(p.out) + b * p.out_bs + h * p.out_hs + col, top == -__builtin_inff() ? 0.f : acc / sum);
+  }
+}
+
+// ------------------------------------------------------------------ host side
+int size_class(const PagedAttnParams &p) {
+  const int most = std::max(p.headdim_k, p.headdim_v);
+  return most <= 64 ? 64 : most <= 128 ? 128 : 256;
+}
+template <typename T, int D> int run(const PagedAttnParams &p, hipStream_t st) {
+  constexpr int V = Frags<T>::V;
+  const int group = p.nheads / p.nkvheads, rows = p.nkvheads * ((group + kHeads - 1) / kHeads);
+  if (rows > 65535 || p.batch > 65535) return MAMBA_E_UNSUPPORTED;
+  const dim3 grid(p.nsplit, rows, p.batch);
+  if (p.headdim_k % V == 0 && p.headdim_v % V == 0) paged_part_kernel<T, D, false><<<grid, kThreads, 0, st>>>(p);
+  else paged_part_kernel<T, D, true><<<grid, kThreads, 0, st>>>(p);
+  if (hipGetLastError() != hipSuccess) return MAMBA_E_LAUNCH;
+  if (p.nsplit > 1) {
+    paged_join_kernel<T, D, Frags<T>::KS><<<dim3(p.nheads, p.batch), kThreads, 0, st>>>(p);
+    if (hipGetLastError() != hipSuccess) return MAMBA_E_LAUNCH;
+  }
+  return MAMBA_OK;
+}
+template <typename T> int run_size(const PagedAttnParams &p, hipStream_t st) {
+  switch (size_class(p)) {
+    case 64: return run<T, 64>(p, st);
+    case 128: return run<T, 128>(p, st);
+    default: return run<T, 256>(p, st);
+  }
+}
+int check(const PagedAttnParams *p) {
+  if (!p) return MAMBA_E_BADARG;
+  if (p->batch <= 0 || p->nheads <= 0 || p->nkvheads <= 0 || p->nheads % p->nkvheads != 0 || p->headdim_k <= 0 || p->headdim_v <= 0)
+    return MAMBA_E_BADARG;
+  if (p->page_size <= 0 || p->num_pages <= 0 || p->max_pages <= 0 || p->window < 0 || p->dtype < MAMBA_F32 || p->dtype > MAMBA_F16)
+    return MAMBA_E_BADARG;
+  if (!(p->scale >= -3.4e38f && p->scale <= 3.4e38f)) return MAMBA_E_BADARG;
+  if (p->headdim_k > 256 || p->headdim_v > 256 || (int64_t)p->max_pages * p->page_size > 1 << 30) return MAMBA_E_UNSUPPORTED;
+  return MAMBA_OK;
+}
+
+}  // namespace
+
+extern "C" int paged_attn_parts(const PagedAttnParams *p) {
+  if (const int rc = check(p)) return rc;
+  const int group = p->nheads / p->nkvheads;
+  const int64_t rows = (int64_t)p->batch * p->nkvheads * ((group + kHeads - 1) / kHeads);
+  const int64_t longest = (int64_t)p->max_pages * p->page_size, most = p->window > 0 ? std::min<int64_t>(p->window, longest) : longest;
+  const int tile = p->dtype == MAMBA_F32 ? 16 : 32;
+  const int64_t parts = std::min<int64_t>((most + 2 * kWaves * tile - 1) / (2 * kWaves * tile), (8 * (int64_t)cu_count() + rows - 1) / rows);
+  return (int)std::max<int64_t>(1, std::min<int64_t>(parts, 1024));
+}
+extern "C" int64_t paged_attn_ws_bytes(const PagedAttnParams *p) {
+  if (const int rc = check(p)) return rc;
+  if (p->nsplit <= 0 || p->nsplit > 65535) return MAMBA_E_BADARG;
+  return p->nsplit == 1 ? 0 : (int64_t)p->batch * p->nheads * p->nsplit * (size_class(*p) + 2) * 4;
+}
+extern "C" int paged_attn_update(const PagedAttnParams *p, mamba_stream_t stream) {
+  if (const int rc = check(p)) return rc;
+  if (!p->q || !p->k_cache || !p->v_cache || !p->block_table || !p->cache_seqlens || !p->out || (p->k == nullptr) != (p->v == nullptr))
+    return MAMBA_E_BADARG;
+  if (p->nsplit <= 0 || p->nsplit > 65535 || (p->nsplit > 1 && (!p->ws || reinterpret_cast<uintptr_t>(p->ws) % 16 != 0))) return MAMBA_E_BADARG;
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  switch (p->dtype) {
+    case MAMBA_F32: return run_size<float>(*p, st);
+    case MAMBA_BF16: return run_size<bf16_t>(*p, st);
+    default: return run_size<f16_t>(*p, st);
+  }
+}

@@ -131,5 +131,6 @@ void bind_norm_conv(pybind11::module_ &m);
 void bind_scan(pybind11::module_ &m);
 void bind_ssd(pybind11::module_ &m);
 void bind_gated(pybind11::module_ &m);
+void bind_attention(pybind11::module_ &m);
 
 }  // namespace mamba_ext

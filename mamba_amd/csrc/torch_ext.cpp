@@ -5,7 +5,8 @@
 // same work takes in Python + ctypes; and the operators' autograd nodes, whose backward passes then run without the
 // interpreter.  This file has the decode-step operators and the module; torch_norm_conv.cpp the norms and the
 // convolution, torch_scan.cpp and torch_ssd.cpp the training operators and the mixers built on them,
-// torch_gated.cpp the gated linear recurrence and the norm between two blocks.
+// torch_gated.cpp the gated linear recurrence and the norm between two blocks, torch_attention.cpp linear attention and the
+// attention over a paged cache.
 // Built as the Python extension module mamba_amd._torch_ext (pybind11), linked against
 // libmamba_gfx950.so; it contains no device code.
 #include "torch_common.h"
@@ -204,4 +205,5 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   bind_scan(m);
   bind_ssd(m);
   bind_gated(m);
+  bind_attention(m);
 }
