@@ -7,11 +7,11 @@ namespace {
 using namespace lin;
 
 // The state of one segment alone, from zero, for the segments behind it.
-template <typename T, int KD, int DVT, bool RAG> __global__ __launch_bounds__(kThreads, KD == 256 ? 1 : 2) void lin_segment_kernel(const LinLaunch p) {
+template <typename T, int KD, int DVT, Fit FIT> __global__ __launch_bounds__(kThreads, (Shape<T, KD, DVT>::WORKGROUPS)) void lin_segment_kernel(const LinLaunch p) {
   using F = Frags<T>;
   using Sh = Shape<T, KD, DVT>;
   constexpr int C = Sh::C;
-  __shared__ __align__(16) typename F::E lb[C * Sh::PK], lc[C * Sh::PV];
+  __shared__ __align__(16) char lds[2][Sh::STAGE];  // (the rows a stay out)
   const Place at = place_of(p);
   if (at.none) return;
   const LinWalk &w = p.w[at.walk];
@@ -19,43 +19,74 @@ template <typename T, int KD, int DVT, bool RAG> __global__ __launch_bounds__(kT
   const int v0 = at.slice * Sh::VAL;
   const Item it = item_of(p, at.item);
   if (v0 >= w.val || it.zero || (it.before + 1) * p.seg_len >= it.len) return;  // the last segment's is not asked for
-  const float l2 = log2_decay(p.log_decay[at.head]);
+  const typename F::template Lane<KD> lanes(i, g, wave % F::NT);
+  const typename F::template ColumnLane<Sh::VAL> values(wave * DVT, i, g);
+  const Decay decay{log2_decay(p.log_decay[at.head])};
   int64_t b_ls, c_ls;
   const T *b = static_cast<const T *>(w.b.p) + rows_at(w.b, it, at.head, w.reverse, p.seg_len, b_ls);
   const T *c = static_cast<const T *>(w.c.p) + rows_at(w.c, it, at.head, w.reverse, p.seg_len, c_ls) + v0;
-  Stage<T, C, KD, RAG> sb;
-  Stage<T, C, Sh::VAL, RAG> sc;
+  Stage<T, C, KD, FIT> sb(b, b_ls, w.key, tid);
+  Stage<T, C, Sh::VAL, FIT> sc(c, c_ls, min(w.val - v0, Sh::VAL), tid);
   WaveState<T, KD, DVT> state;
   state.zero();
-  const int vals = min(w.val - v0, Sh::VAL);
-  sb.fetch(b, b_ls, min(it.n, C), w.key, tid), sc.fetch(c, c_ls, min(it.n, C), vals, tid);
-  for (int t = 0; t < it.n; t += C) {
+  const float write = w.write;
+  const int late = w.late;
+  const Weights<F, Sh::JB, Sh::IT> weights(decay, 0.f, write, late, i, g);
+  auto fetch = [&](int t) {
     const int n = min(it.n - t, C);
-    sb.commit(lb, n, w.key, tid), sc.commit(lc, n, vals, tid);
+    sb.fetch(b + t * b_ls, b_ls, n, tid), sc.fetch(c + t * c_ls, c_ls, n, tid);
+  };
+  auto commit = [&](auto whole, int t, char *rows) {
+    const int n = min(it.n - t, C);
+    sb.template commit<whole.value>(rows + Sh::B, n, tid), sc.template commit<whole.value>(rows + Sh::CC, n, tid);
+  };
+  // whole: so are this block and the next two
+  auto block = [&](auto whole, int t, char *now, char *next) {
+    constexpr bool FULL = whole.value;
+    if (FULL || t + C < it.n) commit(whole, t + C, next);
+    if constexpr (FULL) sb.fetch_next(), sc.fetch_next();
+    else if (t + 2 * C < it.n) fetch(t + 2 * C);
+    state.template update<FULL>(now, lanes, values, decay, weights, write, FULL ? C : min(it.n - t, C), late, g);
     lds_barrier();
-    if (t + C < it.n) {
-      const int next = min(it.n - t - C, C);
-      sb.fetch(b + (t + C) * b_ls, b_ls, next, w.key, tid), sc.fetch(c + (t + C) * c_ls, c_ls, next, vals, tid);
+  };
+  char *now = lds[0], *next = lds[1];
+  const bool steady = FIT != ELEMENTS && it.n >= 3 * C && near(w.b) && near(w.c);
+  int t = 0;
+  if (steady) {
+    sb.fetch_next(), sc.fetch_next();
+    commit(std::true_type{}, 0, now);
+    sb.fetch_next(), sc.fetch_next();
+    lds_barrier();
+    for (; t + 3 * C <= it.n; t += C) {
+      block(std::true_type{}, t, now, next);
+      char *const was = now;
+      now = next, next = was;
     }
-    typename F::Raw cf[Sh::JB][DVT];
-    value_frags<T, KD, DVT>(lc, cf, wave, i, g);
-    state.scale(fast_exp2(l2 * (float)n));
-    state.update(lb, cf, l2, w.write, n - w.late, i, g);
+  } else {
+    fetch(0);
+    commit(std::false_type{}, 0, now);
+    if (C < it.n) fetch(C);
     lds_barrier();
+  }
+#pragma unroll 1
+  for (; t < it.n; t += C) {
+    block(std::false_type{}, t, now, next);
+    char *const was = now;
+    now = next, next = was;
   }
   f32x4 *dst = p.segs + ((((int64_t)at.walk * p.items + at.item) * p.nheads + at.head) * p.slices + at.slice) * (kWaves * Sh::TILES * 64) +
                wave * Sh::TILES * 64 + lane;
   state.each([&](f32x4 &v, int tile) { dst[tile * 64] = v; });
 }
 
-template <typename T, int KD, int DVT, bool RAG> __global__ __launch_bounds__(kThreads, KD == 256 ? 1 : 2) void lin_walk_kernel(const LinLaunch p) {
+// PARTS: there are walks whose y is a part of a sum, in fp32.  (The loop for those beside the other one costs registers that the
+// launches without them need: 8 spilled a block.)
+template <typename T, int KD, int DVT, Fit FIT, bool PARTS> __global__ __launch_bounds__(kThreads, (Shape<T, KD, DVT>::WORKGROUPS)) void lin_walk_kernel(const LinLaunch p) {
   using F = Frags<T>;
   using Sh = Shape<T, KD, DVT>;
-  using E = typename F::E;
+  using Raw = typename F::Raw;
   constexpr int C = Sh::C, KB = Sh::KB, JB = Sh::JB, IT = Sh::IT, NT = F::NT, KS = F::KS, V = F::V;
-  constexpr int BLOCKS = JB * IT;
-  __shared__ __align__(16) E la[C * Sh::PK], lb[C * Sh::PK], lc[C * Sh::PV];
-  __shared__ __align__(16) typename F::Comp lp[BLOCKS][64];
+  __shared__ __align__(16) char lds[Sh::LDS];
   const Place at = place_of(p);
   if (at.none) return;
   const LinWalk &w = p.w[at.walk];
@@ -64,109 +95,131 @@ template <typename T, int KD, int DVT, bool RAG> __global__ __launch_bounds__(kT
   const Item it = item_of(p, at.item);
   if (v0 >= w.val || it.seq < 0) return;
   const int vals = min(w.val - v0, Sh::VAL);
-  // a lane's values of y: NV side by side from value y0 on, per tile or (PAIR) for both
-  constexpr int NV = Sh::PAIR ? 8 : 4, NY = Sh::PAIR ? 1 : DVT;
+
+  // y leaves through LDS, as pieces of whole rows; sums that are still to be added to others leave in fp32 from the registers.
+  // (Stores of a wave's own columns, 32 or 64 bytes a row, save a barrier and cost more: the loop without its products takes 432 us
+  // and not 336 for the backward of 8 x 4096 x 20 x 128.)
   int64_t y_ls;
   const int64_t y_at = rows_at(w.y, it, at.head, w.reverse, p.seg_len, y_ls) + v0;
-  auto put = [&](int64_t row, int d, const float (&v)[NV]) {
-    const int col = wave * Sh::WV + (Sh::PAIR ? 8 * g : 16 * d + 4 * g);
-    if (w.y_f32) {
-      float *dst = static_cast<float *>(w.y.p) + y_at + row * y_ls + col;
+  constexpr int Y_PER = Sh::VAL / V, Y_RUN = kThreads / Y_PER, Y_N = C / Y_RUN;  // pieces of a row, rows of a turn, turns
+  static_assert(C % Y_RUN == 0, "whole turns");
+  const int y_row = tid / Y_PER, y_piece = tid % Y_PER;
+  const bool y_f32 = PARTS && w.y_f32;
+  auto put = [&](T *dst, Raw v) {
+    if constexpr (FIT == ELEMENTS) {
+      typename F::E e[V];
+      __builtin_memcpy(e, &v, 16);
 #pragma unroll
-      for (int e = 0; e < NV; ++e)
-        if (col + e < vals) dst[e] = v[e];
-    } else {
-      T *dst = static_cast<T *>(w.y.p) + y_at + row * y_ls + col;
-      if (!RAG && col + NV <= vals) {
-        if constexpr (std::is_same_v<T, float>) {
-          *(GLOBAL_AS f32x4_a4 *)dst = f32x4{v[0], v[1], v[2], v[3]};
-        } else if constexpr (NV == 8) {
-          st8_any<T>(dst, v);
-        } else {
-          typedef u32x2 u32x2_a2 __attribute__((aligned(2)));
-          if constexpr (DT<T>::id == MAMBA_BF16) *(GLOBAL_AS u32x2_a2 *)dst = u32x2{pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3])};
-          else *(GLOBAL_AS u32x2_a2 *)dst = u32x2{pack_f16(v[0], v[1]), pack_f16(v[2], v[3])};
-        }
-      } else {
+      for (int k = 0; k < V; ++k)
+        if (y_piece * V + k < vals) *reinterpret_cast<typename F::E *>(dst + k) = e[k];
+    } else if (FIT == WHOLE || y_piece * V < vals) {
+      if constexpr (std::is_same_v<T, float>) *(GLOBAL_AS f32x4_a4 *)dst = v;
+      else *(GLOBAL_AS u32x4_a2 *)dst = v;
+    }
+  };
+  auto put_f32 = [&](int64_t row, f32x4 v, int d) {
+    const int value = 16 * (DVT * wave + d) + 4 * g;
+    float *dst = static_cast<float *>(w.y.p) + y_at + row * y_ls + value;
+    if constexpr (FIT == ELEMENTS) {
 #pragma unroll
-        for (int e = 0; e < NV; ++e)
-          if (col + e < vals) st1<T>(dst + e, v[e]);
-      }
+      for (int e = 0; e < 4; ++e)
+        if (value + e < vals) dst[e] = v[e];
+    } else if (FIT == WHOLE || value < vals) {
+      *(GLOBAL_AS f32x4_a4 *)dst = v;
     }
   };
   if (it.zero) {
-    const float zero[NV] = {};
-    for (int row = i; row < it.n; row += 16)
+    if (y_f32) {
+      for (int row = i; row < it.n; row += 16)
 #pragma unroll
-      for (int d = 0; d < NY; ++d) put(row, d, zero);
+        for (int d = 0; d < DVT; ++d) put_f32(row, f32x4{0.f, 0.f, 0.f, 0.f}, d);
+    } else {
+      const Raw none = {};
+      for (int row = y_row; row < it.n; row += Y_RUN) put(static_cast<T *>(w.y.p) + y_at + row * y_ls + y_piece * V, none);
+    }
     return;
   }
 
-  const float l2 = log2_decay(p.log_decay[at.head]);
+  const typename F::template Lane<KD> lanes(i, g, wave % F::NT);
+  const typename F::template ColumnLane<Sh::VAL> values(wave * DVT, i, g);
+  const Decay decay{log2_decay(p.log_decay[at.head])};
   int64_t a_ls, b_ls, c_ls;
   const T *a = static_cast<const T *>(w.a.p) + rows_at(w.a, it, at.head, w.reverse, p.seg_len, a_ls);
   const T *b = static_cast<const T *>(w.b.p) + rows_at(w.b, it, at.head, w.reverse, p.seg_len, b_ls);
   const T *c = static_cast<const T *>(w.c.p) + rows_at(w.c, it, at.head, w.reverse, p.seg_len, c_ls) + v0;
-  Stage<T, C, KD, RAG> sa, sb;
-  Stage<T, C, Sh::VAL, RAG> sc;
+  Stage<T, C, KD, FIT> sa(a, a_ls, w.key, tid), sb(b, b_ls, w.key, tid);
+  Stage<T, C, Sh::VAL, FIT> sc(c, c_ls, vals, tid);
   auto fetch = [&](int t) {
     const int n = min(it.n - t, C);
-    sa.fetch(a + t * a_ls, a_ls, n, w.key, tid), sb.fetch(b + t * b_ls, b_ls, n, w.key, tid), sc.fetch(c + t * c_ls, c_ls, n, vals, tid);
+    sa.fetch(a + t * a_ls, a_ls, n, tid), sb.fetch(b + t * b_ls, b_ls, n, tid), sc.fetch(c + t * c_ls, c_ls, n, tid);
   };
-  if (it.n > 0) fetch(0);
+  auto fetch_next = [&]() { sa.fetch_next(), sb.fetch_next(), sc.fetch_next(); };
+  auto commit = [&](auto whole, int t, char *rows) {
+    const int n = min(it.n - t, C);
+    sa.template commit<whole.value>(rows, n, tid), sb.template commit<whole.value>(rows + Sh::B, n, tid);
+    sc.template commit<whole.value>(rows + Sh::CC, n, tid);
+  };
+  const bool steady = FIT != ELEMENTS && it.n >= 3 * C && near(w.a) && near(w.b) && near(w.c) && near(w.y);
+  if (steady) fetch_next();
+  else if (it.n > 0) fetch(0);
 
   // the state that comes in
   WaveState<T, KD, DVT> state;
   const int64_t seq_head = ((int64_t)it.seq * p.nheads + at.head) * w.key * w.val;
+  const int value = v0 + 16 * DVT * wave + i;
   if (w.start.p) {
-    const float *src = w.start.p + seq_head;
-    state.each_element(i, g, w.key, w.val, v0 + wave * Sh::WV, [&](float, int k, int v, bool ok) {
-      const float x = src[(int64_t)min(k, w.key - 1) * w.start.ks + (int64_t)min(v, w.val - 1) * w.start.vs];
-      return ok ? x : 0.f;
-    });
+    const float *src[DVT];
+#pragma unroll
+    for (int d = 0; d < DVT; ++d) src[d] = w.start.p + seq_head + min(value + 16 * d, w.val - 1) * w.start.vs;
+    state.each_element(g, w.key, [&](float, int d, int k, bool) { return src[d][min(k, w.key - 1) * w.start.ks]; });
+    state.each([](f32x4 &v, int) { asm volatile("" : "+v"(v)); });  // all of them on their way before any is looked at
+    state.each_element(g, w.key, [&](float x, int d, int, bool ok) { return ok && value + 16 * d < w.val ? x : 0.f; });
   } else {
     state.zero();
   }
   if (it.before > 0) {
-    const float f = fast_exp2(l2 * (float)p.seg_len);
+    const float f = decay(p.seg_len);
     const int64_t step = (int64_t)p.nheads * p.slices * (kWaves * Sh::TILES * 64);
     const f32x4 *src = p.segs + (((int64_t)at.walk * p.items + at.item - it.before) * p.nheads * p.slices + at.head * p.slices + at.slice) *
                                     (kWaves * Sh::TILES * 64) + wave * Sh::TILES * 64 + lane;
     for (int s = 0; s < it.before; ++s, src += step) state.each([&](f32x4 &v, int tile) { v = v * f + src[tile * 64]; });
   }
 
-  for (int t = 0; t < it.n; t += C) {
-    const int n = min(it.n - t, C);
-    sa.commit(la, n, w.key, tid), sb.commit(lb, n, w.key, tid), sc.commit(lc, n, vals, tid);
-    lds_barrier();
-    if (t + C < it.n) fetch(t + C);
-    // (a_t . b_s) f^(t - s), the blocks of KS s on and below the diagonal in turn by the waves
-    int f = 0;
+  const float read = w.read, write = w.write;
+  const int late = w.late;
+  const Weights<F, JB, IT> weights(decay, read, write, late, i, g);
+  // (a_t . b_s) f^(t - s) mix: a wave has a tile of 16 t and half of KS s, of those blocks that reach the diagonal
+  const int tile = wave / NT, half = wave % NT;
+  int ib_of = 0, jb_of = tile;
+  for (int per = 1; jb_of >= per; ++ib_of, per = (16 * ib_of + 15) / KS + 1) jb_of -= per;
+  const int first = 16 * ib_of + i - (KS * jb_of + F::krow(4 * g, half));  // t - s of the lane's first s
+  float pair[4];
 #pragma unroll
-    for (int ib = 0; ib < IT; ++ib)
+  for (int r = 0; r < 4; ++r) pair[r] = w.mix * decay(max(first - r, 0));
+  auto scores = [&](const char *rows, char *to) {
+    if (tile >= Sh::BLOCKS) return;
+    const char *ar = rows + F::size(16 * ib_of, KD), *br = rows + Sh::B + F::size(KS * jb_of, KD);
+    f32x4 acc = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int jb = 0; jb < JB; ++jb) {
-        if (jb * KS > ib * 16 + 15) continue;
-        if ((f++ & 3) != wave) continue;
-        f32x4 acc[NT];
+    for (int kb = 0; kb < KB; ++kb) acc = F::mma_raw(lanes.along_krow(br, kb), lanes.along(ar, kb), acc);
 #pragma unroll
-        for (int h = 0; h < NT; ++h) acc[h] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int kb = 0; kb < KB; ++kb) {
-          const auto ar = F::along(la + (16 * ib + i) * Sh::PK + KS * kb + V * g);
-#pragma unroll
-          for (int h = 0; h < NT; ++h)
-            acc[h] = F::mma_raw(F::along(lb + (KS * jb + F::krow(i, h)) * Sh::PK + KS * kb + V * g), ar, acc[h]);
-        }
-        float v[V];
-        F::gather(acc, v);
-#pragma unroll
-        for (int e = 0; e < V; ++e) {
-          const int apart = 16 * ib + i - (KS * jb + V * g + e);
-          v[e] = apart >= 0 ? v[e] * (w.mix * fast_exp2(l2 * (float)apart)) : 0.f;
-        }
-        lp[ib * JB + jb][lane] = F::comp(v);
-      }
+    for (int r = 0; r < 4; ++r) acc[r] = r <= first ? acc[r] * pair[r] : 0.f;
+    F::store_comp(reinterpret_cast<typename F::Comp *>(to) + tile * 64 + lane, half, acc);
+  };
+
+  // whole blocks of near rows: the lowest row of a turn, from turn to turn, the thread's place (bytes)
+  char *y_low = uniform_pointer(static_cast<char *>(w.y.p) + (y_at + (y_ls < 0 ? (Y_RUN - 1) * y_ls : 0)) * (int64_t)sizeof(T));
+  const int64_t y_run = Y_RUN * y_ls * (int64_t)sizeof(T);
+  const uint32_t y_place = (uint32_t)((y_ls < 0 ? Y_RUN - 1 - y_row : y_row) * (int)(y_ls < 0 ? -y_ls : y_ls) + y_piece * V) * (uint32_t)sizeof(T);
+  // One block: rows in `now`, scores in `s_now`; the next one's rows are laid down, its scores formed, those of the one behind it asked
+  // for.  whole: so are all three; then f32 has to be known as well: loads and stores are counted together, and where the number of
+  // stores behind a block's loads depends on a branch, waiting for the loads waits for the stores too.
+  auto block = [&](auto whole, auto f32, int t, char *now, char *next, const char *s_now, char *s_next) {
+    constexpr bool FULL = whole.value;
+    const int n = FULL ? C : min(it.n - t, C);
+    if (FULL || t + C < it.n) commit(whole, t + C, next);
+    if constexpr (FULL) fetch_next();
+    else if (t + 2 * C < it.n) fetch(t + 2 * C);
     // y from the state that came in
     f32x4 y[IT][DVT];
 #pragma unroll
@@ -178,62 +231,94 @@ template <typename T, int KD, int DVT, bool RAG> __global__ __launch_bounds__(kT
       typename F::Comp s[DVT];
 #pragma unroll
       for (int d = 0; d < DVT; ++d) {
-        f32x4 tiles[NT];
-#pragma unroll
-        for (int h = 0; h < NT; ++h) tiles[h] = state.t[kb][h][d];
         float v[V];
-        F::gather(tiles, v);
+        F::gather(state.t[d][kb], v);
         s[d] = F::comp(v);
       }
 #pragma unroll
       for (int ib = 0; ib < IT; ++ib) {
-        const auto ar = F::data(F::along(la + (16 * ib + i) * Sh::PK + KS * kb + V * g));
+        const typename F::Data ad = F::data(lanes.along(now + F::size(16 * ib, KD), kb));
 #pragma unroll
-        for (int d = 0; d < DVT; ++d) y[ib][d] = mma16(s[d], ar, y[ib][d]);
+        for (int d = 0; d < DVT; ++d) y[ib][d] = mma16(s[d], ad, y[ib][d]);
       }
     }
 #pragma unroll
     for (int ib = 0; ib < IT; ++ib) {
-      const float f = w.read * fast_exp2(l2 * (float)(16 * ib + i + w.late));
+      const float in = FULL ? weights.in_lane * weights.in_block[ib] : read * decay(16 * ib + i + late);
 #pragma unroll
-      for (int d = 0; d < DVT; ++d) y[ib][d] *= f;
+      for (int d = 0; d < DVT; ++d) y[ib][d] *= in;
     }
-    typename F::Raw cf[JB][DVT];
-    value_frags<T, KD, DVT>(lc, cf, wave, i, g);
-    state.scale(fast_exp2(l2 * (float)n));
-    state.update(lb, cf, l2, w.write, n - w.late, i, g);
-    lds_barrier();  // nothing of the block's rows is read behind this
 #pragma unroll
     for (int jb = 0; jb < JB; ++jb) {
       typename F::Data cd[DVT];
 #pragma unroll
-      for (int d = 0; d < DVT; ++d) cd[d] = F::data(cf[jb][d]);
+      for (int d = 0; d < DVT; ++d) cd[d] = F::data(values.columns(now + Sh::CC + F::size(KS * jb, Sh::VAL), d));
 #pragma unroll
       for (int ib = 0; ib < IT; ++ib) {
         if (jb * KS > ib * 16 + 15) continue;
-        const typename F::Comp pf = lp[ib * JB + jb][lane];
+        const typename F::Comp s = reinterpret_cast<const typename F::Comp *>(s_now)[Sh::block_of(ib, jb) * 64 + lane];
 #pragma unroll
-        for (int d = 0; d < DVT; ++d) y[ib][d] = mma16(cd[d], pf, y[ib][d]);
+        for (int d = 0; d < DVT; ++d) y[ib][d] = mma16(cd[d], s, y[ib][d]);
       }
     }
 #pragma unroll
-    for (int ib = 0; ib < IT; ++ib) {
-      const int row = 16 * ib + i;
-      if (row < n) {
+    for (int ib = 0; ib < IT; ++ib)
 #pragma unroll
-        for (int d = 0; d < NY; ++d) {
-          float v[NV];
+      for (int d = 0; d < DVT; ++d) {
+        if (!f32) F::template store<Sh::VAL>(lds + Sh::AT_Y, 16 * ib + i, DVT * wave + d, g, y[ib][d]);
+        else if (FULL || 16 * ib + i < n) put_f32(t + 16 * ib + i, y[ib][d], d);
+      }
+    lds_barrier();
+    if (!f32) {
 #pragma unroll
-          for (int e = 0; e < NV; ++e) v[e] = Sh::PAIR ? y[ib][e >> 2][e & 3] : y[ib][d][e & 3];
-          put(t + row, d, v);
+      for (int q = 0; q < Y_N; ++q) {
+        const int row = q * Y_RUN + y_row;
+        const Raw v = *reinterpret_cast<const Raw *>(lds + Sh::AT_Y + (int)sizeof(typename F::E) * F::template place<Sh::VAL>(row, y_piece));
+        if constexpr (FULL) {
+          asm("" : "+s"(y_low));
+          put(reinterpret_cast<T *>(y_low + y_place), v);
+          y_low += y_run;
+        } else if (row < n) {
+          put(static_cast<T *>(w.y.p) + y_at + (t + row) * y_ls + y_piece * V, v);
         }
       }
     }
+    state.template update<FULL>(now, lanes, values, decay, weights, write, n, late, g);
+    if (FULL || t + C < it.n) scores(next, s_next);
+    lds_barrier();
+  };
+  char *now = lds, *next = lds + Sh::STAGE, *s_now = lds + Sh::AT_SCORES, *s_next = s_now + Sh::SCORES;
+  auto turn_over = [&]() {
+    char *const was = now, *const s_was = s_now;
+    now = next, next = was, s_now = s_next, s_next = s_was;
+  };
+  int t = 0;
+  if (it.n > 0) {
+    if (steady) {
+      commit(std::true_type{}, 0, now);
+      fetch_next();
+    } else {
+      commit(std::false_type{}, 0, now);
+      if (C < it.n) fetch(C);
+    }
+    lds_barrier();
+    scores(now, s_now);
+    lds_barrier();
   }
+  auto steady_blocks = [&](auto f32) {
+    for (; t + 3 * C <= it.n; t += C) block(std::true_type{}, f32, t, now, next, s_now, s_next), turn_over();
+  };
+  if (steady) {
+    if constexpr (PARTS)
+      if (y_f32) steady_blocks(std::true_type{});
+    steady_blocks(std::false_type{});  // (none are left behind the others)
+  }
+#pragma unroll 1
+  for (; t < it.n; t += C) block(std::false_type{}, y_f32, t, now, next, s_now, s_next), turn_over();
   if (w.end.p && (it.before + 1) * (int64_t)p.seg_len >= it.len) {
-    float *dst = w.end.p + seq_head;
-    state.each_element(i, g, w.key, w.val, v0 + wave * Sh::WV, [&](float x, int k, int v, bool ok) {
-      if (ok) dst[(int64_t)k * w.end.ks + (int64_t)v * w.end.vs] = x;
+    float *dst = w.end.p + seq_head + value * w.end.vs;
+    state.each_element(g, w.key, [&](float x, int d, int k, bool ok) {
+      if (ok && value + 16 * d < w.val) dst[16 * d * w.end.vs + k * w.end.ks] = x;
       return x;
     });
   }
@@ -302,10 +387,11 @@ template <typename T> __global__ __launch_bounds__(kThreads) void lin_shared_ker
 
 // ------------------------------------------------------------------ host side
 // How a pass is cut: the sizes that the kernels are made for, the values of a workgroup, and segments of a sequence where
-// there are too few (sequence, head, slice) walks for the chip.
+// there are fewer (sequence, head, slice) walks than the chip has room for.
 struct Cut {
-  int kd, dvt, slices, nseg, seg_len, items;
-  bool ragged, packed;
+  int kd, tiles, slices, nseg, seg_len, items;
+  Fit fit;
+  bool packed;
   int64_t state_bytes, plan_bytes;
 };
 Cut cut_of(const LinearAttnParams &p, int nwalks) {
@@ -313,47 +399,72 @@ Cut cut_of(const LinearAttnParams &p, int nwalks) {
   const int most = p.headdim_k > p.headdim_v ? p.headdim_k : p.headdim_v, v = p.dtype == MAMBA_F32 ? 4 : 8;
   const int val = nwalks == 1 ? p.headdim_v : most, key = nwalks == 1 ? p.headdim_k : most;
   c.kd = key <= 64 ? 64 : key <= 128 ? 128 : 256;
-  c.dvt = val > 64 && c.kd <= 128 && p.dtype != MAMBA_F16 ? 2 : 1;  // (two tiles of values more would not fit the registers)
-  c.slices = (val + 64 * c.dvt - 1) / (64 * c.dvt);
-  c.ragged = p.headdim_k % v != 0 || p.headdim_v % v != 0;
   c.packed = p.nseq > 0;
-  const int64_t seqs = c.packed ? p.nseq : p.batch, walks = (int64_t)p.nheads * c.slices * nwalks;
-  const int64_t total = (int64_t)p.batch * p.seqlen, room = 2 * cu_count();
-  // positions of a segment: as many as make every workgroup's share of the chip, four blocks at least
-  const int64_t share = (total * walks + room - 1) / room, least = 256;
-  int64_t len = (std::max(share, least) + 63) / 64 * 64;
-  const int64_t longest = c.packed ? total : p.seqlen;
-  if (seqs * walks >= room / 2 * (c.packed ? 2 : 1) || len >= longest) len = longest;
-  c.nseg = (int)((longest + len - 1) / len);
-  if (c.nseg < 1) c.nseg = 1;
+  const int64_t seqs = c.packed ? p.nseq : p.batch, chains = (int64_t)p.nheads * nwalks, cus = cu_count();
+  const int64_t total = (int64_t)p.batch * p.seqlen, longest = c.packed ? total : p.seqlen;
+  // Segments of 128 positions at least: of 64, every segment's own state and the sum of those before it cost as much as the walk
+  // (a row of 777 in bf16, 24 heads: 29 us with 128 and 30 with 64; 2048 in fp32: 38 and 48, 41 with 256).
+  constexpr int64_t kLeast = 128;
+  // Two tiles of 16 values a wave read a block's rows once for both (8 x 4096 x 20 x 128, backward: 454 us, 510 with one) as long as there are
+  // workgroups for the chip with them (that row of 777: 38 us with two, 29 with one).
+  const int64_t pieces = c.packed ? seqs + total / kLeast : seqs * std::max<int64_t>(p.seqlen / kLeast, 1);
+  c.tiles = val > 64 && c.kd <= 128 && pieces * chains * ((val + 127) / 128) >= cus ? 2 : 1;
+  const int values_of = 64 * c.tiles;
+  c.slices = (val + values_of - 1) / values_of;
+  const bool keys = p.headdim_k == c.kd && (nwalks == 1 || p.headdim_v == c.kd);
+  const bool values = p.headdim_v % values_of == 0 && (nwalks == 1 || p.headdim_k % values_of == 0);
+  c.fit = p.headdim_k % v != 0 || p.headdim_v % v != 0 ? ELEMENTS : keys && values ? WHOLE : PIECES;
+  // Whole sequences where their walks fill the chip, as the segments' states are one more pass over half of what is read (8 x 4096 x
+  // 20 x 128, backward: 454 us in one piece, 585 in two); else as many segments as fill it once (forward, 160 walks for 512 places: 250
+  // us in three pieces, 264 in four, 257 in one).  Packed sequences may be of any length: segments of an even share.
+  const int64_t walks = chains * c.slices, slots = cus * (c.kd == 256 ? 1 : c.kd == 128 ? 2 : 4);
+  int64_t len = longest;
+  if (seqs * walks < slots) {
+    const int64_t most = std::max<int64_t>(p.seqlen / kLeast, 1), n = std::min(slots / (seqs * walks), most);
+    len = c.packed ? std::max(total * walks / slots, kLeast) : (p.seqlen + n - 1) / n;
+    len = (len + 31) / 32 * 32;
+  }
+  c.nseg = (int)std::max<int64_t>((longest + len - 1) / len, 1);
   c.seg_len = c.nseg == 1 ? INT32_MAX : (int)len;
   c.items = c.packed ? (int)(seqs + 2 + (c.nseg > 1 ? total / len : 0)) : (int)(seqs * c.nseg);
   c.plan_bytes = c.packed && c.nseg > 1 ? ((int64_t)c.items + 1) * 16 : 0;
-  c.state_bytes = c.nseg > 1 ? (int64_t)nwalks * c.items * p.nheads * c.slices * c.kd * 64 * c.dvt * 4 : 0;
+  c.state_bytes = c.nseg > 1 ? (int64_t)nwalks * c.items * p.nheads * c.slices * c.kd * values_of * 4 : 0;
   return c;
 }
 
-template <typename T, int KD, int DVT, bool RAG> int run(const LinLaunch &l, hipStream_t st) {
+template <typename T, int KD, int DVT, Fit FIT> int run(const LinLaunch &l, hipStream_t st) {
   const int64_t outer = ((int64_t)l.items * l.kv_heads + 7) / 8 * 8, blocks = outer * (l.nheads / l.kv_heads) * l.nwalks * l.slices;
   if (blocks > INT32_MAX) return MAMBA_E_UNSUPPORTED;
   if (l.nseg > 1) {
-    lin_segment_kernel<T, KD, DVT, RAG><<<(int)blocks, kThreads, 0, st>>>(l);
+    lin_segment_kernel<T, KD, DVT, FIT><<<(int)blocks, kThreads, 0, st>>>(l);
     if (hipGetLastError() != hipSuccess) return MAMBA_E_LAUNCH;
   }
-  lin_walk_kernel<T, KD, DVT, RAG><<<(int)blocks, kThreads, 0, st>>>(l);
+  if constexpr (sizeof(T) < 4) {
+    if (l.w[l.nwalks - 1].y_f32) {
+      lin_walk_kernel<T, KD, DVT, FIT, true><<<(int)blocks, kThreads, 0, st>>>(l);
+      return hipGetLastError() == hipSuccess ? MAMBA_OK : MAMBA_E_LAUNCH;
+    }
+  }
+  lin_walk_kernel<T, KD, DVT, FIT, false><<<(int)blocks, kThreads, 0, st>>>(l);
   return hipGetLastError() == hipSuccess ? MAMBA_OK : MAMBA_E_LAUNCH;
 }
-template <typename T, int KD> int run_dvt(const LinLaunch &l, const Cut &c, hipStream_t st) {
-  if constexpr (KD <= 128 && !std::is_same_v<T, f16_t>) {
-    if (c.dvt == 2) return c.ragged ? run<T, KD, 2, true>(l, st) : run<T, KD, 2, false>(l, st);
+template <typename T, int KD, int DVT> int run_fit(const LinLaunch &l, const Cut &c, hipStream_t st) {
+  switch (c.fit) {
+    case WHOLE: return run<T, KD, DVT, WHOLE>(l, st);
+    case PIECES: return run<T, KD, DVT, PIECES>(l, st);
+    default: return run<T, KD, DVT, ELEMENTS>(l, st);
   }
-  return c.ragged ? run<T, KD, 1, true>(l, st) : run<T, KD, 1, false>(l, st);
+}
+template <typename T, int KD> int run_tiles(const LinLaunch &l, const Cut &c, hipStream_t st) {
+  if constexpr (KD <= 128)
+    if (c.tiles == 2) return run_fit<T, KD, 2>(l, c, st);
+  return run_fit<T, KD, 1>(l, c, st);
 }
 template <typename T> int run_kd(const LinLaunch &l, const Cut &c, hipStream_t st) {
   switch (c.kd) {
-    case 64: return run_dvt<T, 64>(l, c, st);
-    case 128: return run_dvt<T, 128>(l, c, st);
-    default: return run_dvt<T, 256>(l, c, st);
+    case 64: return run_tiles<T, 64>(l, c, st);
+    case 128: return run_tiles<T, 128>(l, c, st);
+    default: return run_tiles<T, 256>(l, c, st);
   }
 }
 int run_type(const LinLaunch &l, const Cut &c, int dtype, hipStream_t st) {

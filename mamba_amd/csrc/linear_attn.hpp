@@ -103,20 +103,54 @@ DEVI float log2_decay(float l) {
   return (l < -1e6f ? -1e6f : l) * kLog2e;
 }
 
-// C rows x COLS columns of a tensor on their way to LDS, in pieces of 16 bytes; rows from n on and columns from `cols` on
-// become 0.  RAG: `cols` may be any number.
-template <typename T, int C, int COLS, bool RAG> struct Stage {
+// Rows less than 2^22 elements apart are read through uniform pointers and 32-bit places of the lanes.
+constexpr int64_t kNear = 1 << 22;
+DEVI bool near(const LinRows &r) { return r.ls <= kNear && r.ls >= -kNear; }
+
+// the same pointer, in scalar registers
+template <typename P> DEVI P *uniform_pointer(P *p) {
+  const uint64_t a = reinterpret_cast<uint64_t>(p);
+  const uint32_t lo = __builtin_amdgcn_readfirstlane((uint32_t)a), hi = __builtin_amdgcn_readfirstlane((uint32_t)(a >> 32));
+  return reinterpret_cast<P *>((uint64_t)hi << 32 | lo);
+}
+
+// How the head sizes lie in those that a kernel is made for: they are those; whole pieces of 16 bytes less; any number less, read
+// element by element.
+enum Fit { WHOLE, PIECES, ELEMENTS };
+
+// C rows x COLS columns of a tensor on their way to LDS, in pieces of 16 bytes; rows from n on and columns from `cols` on become 0.
+template <typename T, int C, int COLS, Fit FIT> struct Stage {
   using F = Frags<T>;
-  static constexpr int V = F::V, PER = COLS / V, N = C * PER / kThreads, PITCH = COLS + F::PAD;
-  static_assert(C * PER % kThreads == 0, "whole pieces per thread");
+  static constexpr int V = F::V, PER = COLS / V, N = C * PER / kThreads, RUN = kThreads / PER;  // rows of a turn
+  static_assert(C * PER % kThreads == 0 && kThreads % PER == 0, "whole pieces per thread");
   using Raw = typename F::Raw;
   Raw w[N];
-  DEVI void fetch(const T *at, int64_t ls, int n, int cols, int tid) {
+  // whole blocks of near rows: where the next block's lowest row lies, bytes from a turn's rows to the next's and from block to block, the
+  // thread's place
+  const char *low;
+  int64_t run, step;
+  uint32_t place;
+  int cols, lds;  // lds: of the piece in the tile
+  DEVI Stage(const T *first, int64_t ls, int cols_, int tid) : cols(cols_), lds((int)sizeof(typename F::E) * F::template place<COLS>(tid / PER, tid % PER)) {
+    const int row = tid / PER;
+    const bool back = ls < 0;
+    low = uniform_pointer(reinterpret_cast<const char *>(back ? first + (RUN - 1) * ls : first));  // a turn's rows lie from here on
+    run = RUN * ls * (int64_t)sizeof(T), step = C * ls * (int64_t)sizeof(T);
+    place = (uint32_t)((back ? RUN - 1 - row : row) * (int)(back ? -ls : ls) + (FIT == WHOLE ? tid % PER * V : FIT == PIECES ? min(tid % PER * V, cols - V) : 0)) * (uint32_t)sizeof(T);
+  }
+  DEVI void fetch_next() {
+    asm("" : "+s"(low));  // (it stays a scalar: one register of offsets and no 64-bit sums in the lanes)
+#pragma unroll
+    for (int q = 0; q < N; ++q) w[q] = any(reinterpret_cast<const T *>(low + q * run + place));
+    low += step;
+  }
+  // `at`: the block's first row, ls: to the next one
+  DEVI void fetch(const T *at, int64_t ls, int n, int tid) {
 #pragma unroll
     for (int q = 0; q < N; ++q) {
       const int id = q * kThreads + tid, row = min(id / PER, n - 1), col = id % PER * V;
       const T *src = at + (int64_t)row * ls;
-      if constexpr (RAG) {
+      if constexpr (FIT == ELEMENTS) {
         typename F::E v[V];
 #pragma unroll
         for (int e = 0; e < V; ++e) v[e] = *(const GLOBAL_AS typename F::E *)(src + min(col + e, cols - 1));
@@ -126,23 +160,25 @@ template <typename T, int C, int COLS, bool RAG> struct Stage {
       }
     }
   }
-  DEVI void commit(typename F::E *lds, int n, int cols, int tid) const {
+  template <bool FULL> DEVI void commit(char *tile, int n, int tid) const {
 #pragma unroll
     for (int q = 0; q < N; ++q) {
       const int id = q * kThreads + tid, row = id / PER, col = id % PER * V;
       Raw v = w[q];
-      if constexpr (RAG) {
+      if constexpr (FIT == ELEMENTS) {
         typename F::E e[V];
         __builtin_memcpy(e, &v, 16);
 #pragma unroll
         for (int k = 0; k < V; ++k) e[k] = row < n && col + k < cols ? e[k] : typename F::E(0);
         __builtin_memcpy(&v, e, 16);
-      } else {
-        const bool ok = row < n && col < cols;
+      } else if constexpr (!FULL || FIT == PIECES) {
+        const bool ok = (FULL || row < n) && (FIT == WHOLE || col < cols);
 #pragma unroll
         for (int k = 0; k < 4; ++k) v[k] = ok ? v[k] : 0;
       }
-      *reinterpret_cast<Raw *>(lds + row * PITCH + col) = v;
+      // (the order of a row's pieces repeats every 16 rows)
+      const int at = RUN % 16 == 0 ? lds + F::size(q * RUN, COLS) : (int)sizeof(typename F::E) * F::template place<COLS>(row, id % PER);
+      *reinterpret_cast<Raw *>(tile + at) = v;
     }
   }
   static DEVI Raw any(const T *at) {
@@ -151,93 +187,122 @@ template <typename T, int C, int COLS, bool RAG> struct Stage {
   }
 };
 
+// A workgroup of 4 waves, DVT tiles of 16 values each: its state (KD keys) lies in their registers, the rows of a block of C positions
+// and of the next one in LDS.
 template <typename T, int KD, int DVT> struct Shape {
   using F = Frags<T>;
-  static constexpr int C = std::is_same_v<T, float> ? 32 : 64;  // positions of a block
+  // (16 positions of fp32 rows: two stages of 32 leave room for one workgroup or none)
+  static constexpr int C = sizeof(T) == 4 ? 16 : 32;
   static constexpr int KB = KD / F::KS, JB = C / F::KS, IT = C / 16;
-  static constexpr int WV = 16 * DVT, VAL = kWaves * WV;         // values of a wave, of a workgroup
-  static constexpr int TILES = KB * F::NT * DVT;                 // tiles of a wave's state
-  static constexpr bool PAIR = F::NT == 2 && DVT == 2;           // a lane's 8 values lie side by side
-  static constexpr int PK = KD + F::PAD, PV = VAL + F::PAD;
+  static constexpr int VAL = 64 * DVT;
+  static constexpr int TILES = DVT * KB * F::NT;  // tiles of a wave's state
+  // blocks of 16 t and KS s that have an s <= t, row by row
+  static constexpr int block_of(int ib, int jb) {
+    int n = 0;
+    for (int r = 0; r < ib; ++r) n += (16 * r + 15) / F::KS + 1;
+    return n + jb;
+  }
+  static constexpr int BLOCKS = block_of(IT, 0);
+  static_assert(BLOCKS * F::NT <= kWaves, "a tile of scores a wave");
+  // LDS, bytes: rows a, b, c of a stage, two of them; decayed scores, twice; y
+  static constexpr int B = F::size(C, KD), CC = 2 * B, STAGE = CC + F::size(C, VAL);
+  static constexpr int SCORES = BLOCKS * 64 * (int)sizeof(typename F::Comp), AT_SCORES = 2 * STAGE, AT_Y = AT_SCORES + 2 * SCORES;
+  static constexpr int LDS = AT_Y + F::size(C, VAL);
+  // workgroups of a CU: what the LDS has room for and what the registers hold without spills (128, 256 or 512 a lane)
+  static constexpr int ROOM = 160 * 1024 / LDS, MOST = TILES <= 4 ? 4 : KD <= 128 ? 2 : 1;
+  static constexpr int WORKGROUPS = ROOM < 1 ? 1 : ROOM < MOST ? ROOM : MOST;
 };
 
-// ---- the state of a wave: tile (kb, half, d) has keys KS kb + krow(m, half) and values value(n, d)
+// f^n = 2^(n l2) of a head
+struct Decay {
+  float l2;
+  DEVI float operator()(int n) const { return fast_exp2(l2 * (float)n); }
+  DEVI float uniform(int n) const { return __builtin_bit_cast(float, __builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, (*this)(n)))); }
+};
+// What the whole blocks of a walk are weighted with: products of what a lane and what an element has of f^n, neither above 1.
+template <typename F, int JB, int IT> struct Weights {
+  float in_lane, in_block[IT];                    // read f^(16 ib + i + late) of y's rows
+  float up_lane, up_element[F::V], up_block[JB];  // write f^(last - KS jb - V g - e) of c's rows
+  float keep;                                     // f^C
+  DEVI Weights(const Decay &f, float read, float write, int late, int i, int g) {
+    in_lane = read * f(i + late);
+    up_lane = write * f(F::V * (3 - g) + (1 - late));  // last = C - late, the last block's last group: f^(C - late - (C - 4 V + V g + V - 1))
+#pragma unroll
+    for (int n = 0; n < IT; ++n) in_block[n] = f.uniform(16 * n);
+#pragma unroll
+    for (int n = 0; n < JB; ++n) up_block[n] = f.uniform(F::KS * (JB - 1 - n));
+#pragma unroll
+    for (int e = 0; e < F::V; ++e) up_element[e] = f.uniform(F::V - 1 - e);
+    keep = f.uniform(F::KS * JB);
+  }
+};
+
+// ---- the state of a wave: lane (i, g) of tile (d, kb, half) has the keys KS kb + krow(4 g + r, half) of value 16 d + i
 template <typename T, int KD, int DVT> struct WaveState {
   using F = Frags<T>;
   using Sh = Shape<T, KD, DVT>;
-  f32x4 t[Sh::KB][F::NT][DVT];
-  static DEVI int value(int i, int d) { return Sh::PAIR ? 8 * (i >> 2) + (i & 3) + 4 * d : 16 * d + i; }
+  using Values = typename F::template ColumnLane<Sh::VAL>;
+  f32x4 t[DVT][Sh::KB][F::NT];
+  template <typename G> DEVI void each(G f) {
+#pragma unroll
+    for (int d = 0; d < DVT; ++d)
+#pragma unroll
+      for (int kb = 0; kb < Sh::KB; ++kb)
+#pragma unroll
+        for (int h = 0; h < F::NT; ++h) f(t[d][kb][h], (d * Sh::KB + kb) * F::NT + h);
+  }
   DEVI void zero() {
     each([](f32x4 &v, int) { v = f32x4{0.f, 0.f, 0.f, 0.f}; });
   }
-  template <typename G> DEVI void each(G f) {
+  // x = f(x, tile of values, key, whether there is such a key) for every element
+  template <typename G> DEVI void each_element(int g, int key, G f) {
 #pragma unroll
-    for (int kb = 0; kb < Sh::KB; ++kb)
+    for (int d = 0; d < DVT; ++d)
 #pragma unroll
-      for (int h = 0; h < F::NT; ++h)
+      for (int kb = 0; kb < Sh::KB; ++kb)
 #pragma unroll
-        for (int d = 0; d < DVT; ++d) f(t[kb][h][d], (kb * F::NT + h) * DVT + d);
-  }
-  // x = f(x, key, value, whether there is such a place in memory) for every element
-  template <typename G> DEVI void each_element(int i, int g, int key, int val, int v0, G f) {
-#pragma unroll
-    for (int kb = 0; kb < Sh::KB; ++kb)
-#pragma unroll
-      for (int h = 0; h < F::NT; ++h)
-#pragma unroll
-        for (int d = 0; d < DVT; ++d)
+        for (int h = 0; h < F::NT; ++h)
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
-            const int k = F::KS * kb + F::krow(4 * g + r, h), v = v0 + value(i, d);
-            t[kb][h][d][r] = f(t[kb][h][d][r], k, v, k < key && v < val);
+            const int k = F::KS * kb + F::krow(4 * g + r, h);
+            t[d][kb][h][r] = f(t[d][kb][h][r], d, k, k < key);
           }
   }
-  DEVI void scale(float f) {
-    each([&](f32x4 &v, int) { v *= f; });
-  }
-  // + write b^T diag(f^(n - late - s)) c over the block's positions
-  DEVI void update(const typename F::E *b, const typename F::Raw (&cf)[Sh::JB][DVT], float l2, float write, int last, int i, int g) {
+  // f^n Z + write b^T diag(f^(n - late - s)) c over the n positions of a stage's rows
+  template <bool FULL, typename WT>
+  DEVI void update(const char *rows, const typename F::template Lane<KD> &lanes, const Values &values, const Decay &f, const WT &weights, float write, int n, int late,
+                   int g) {
     constexpr int V = F::V;
+    const float keep = FULL ? weights.keep : f(n);
+    each([&](f32x4 &v, int) { v *= keep; });
 #pragma unroll
     for (int jb = 0; jb < Sh::JB; ++jb) {
-      float f[V];
-#pragma unroll
-      for (int e = 0; e < V; ++e) f[e] = write * fast_exp2(l2 * (float)max(last - (F::KS * jb + V * g + e), 0));
       typename F::Wide wc[DVT];
 #pragma unroll
       for (int d = 0; d < DVT; ++d) {
         float v[V];
-        F::unpack(cf[jb][d], v);
+        F::unpack(values.columns(rows + Sh::CC + F::size(F::KS * jb, Sh::VAL), d), v);
+        if constexpr (FULL) {
+          const float lane = weights.up_lane * weights.up_block[jb];
 #pragma unroll
-        for (int e = 0; e < V; ++e) v[e] *= f[e];
+          for (int e = 0; e < V; ++e) v[e] = v[e] * weights.up_element[e] * lane;
+        } else {
+#pragma unroll
+          for (int e = 0; e < V; ++e) v[e] *= write * f(max(n - late - (F::KS * jb + V * g + e), 0));
+        }
         wc[d] = F::wide(v);
       }
 #pragma unroll
       for (int kb = 0; kb < Sh::KB; ++kb)
 #pragma unroll
         for (int h = 0; h < F::NT; ++h) {
-          const auto bt = F::data(F::template columns<Sh::PK>(b + F::KS * jb * Sh::PK, F::KS * kb, h, i, g));
+          const typename F::Data b = F::data(lanes.columns(rows + Sh::B + F::size(F::KS * jb, KD), kb, h));
 #pragma unroll
-          for (int d = 0; d < DVT; ++d) t[kb][h][d] = mma16(bt, wc[d], t[kb][h][d]);
+          for (int d = 0; d < DVT; ++d) t[d][kb][h] = mma16(b, wc[d], t[d][kb][h]);
         }
     }
   }
 };
-
-// c^T fragments of the block for a wave's values
-template <typename T, int KD, int DVT>
-DEVI void value_frags(const typename Frags<T>::E *c, typename Frags<T>::Raw (&cf)[Shape<T, KD, DVT>::JB][DVT], int wave, int i, int g) {
-  using F = Frags<T>;
-  using Sh = Shape<T, KD, DVT>;
-#pragma unroll
-  for (int jb = 0; jb < Sh::JB; ++jb)
-#pragma unroll
-    for (int d = 0; d < DVT; ++d) {
-      const auto *at = c + F::KS * jb * Sh::PV;
-      if constexpr (Sh::PAIR) cf[jb][d] = F::template columns<Sh::PV>(at, wave * Sh::WV, d, i, g);
-      else cf[jb][d] = F::template columns_in_order<Sh::PV>(at, wave * Sh::WV + 16 * d, i, g);
-    }
-}
 
 // Element (first position of the segment, 0) of a tensor's head, and the step from one position of the walk to the next.
 DEVI int64_t rows_at(const LinRows &r, const Item &it, int head, int reverse, int seg_len, int64_t &ls) {

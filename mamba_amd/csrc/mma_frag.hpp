@@ -57,22 +57,50 @@ DEVI frag_i16x4 lds_transposed(const uint16_t *src) {
 
 template <typename T> struct Frags16 {
   using E = uint16_t;  // as it lies in LDS
-  static constexpr int KS = 32, NT = 2, V = 8, PAD = 8;
+  static constexpr int KS = 32, NT = 2, V = 8;
   static DEVI int krow(int m, int half) { return 8 * (m >> 2) + (m & 3) + 4 * half; }
-  // row i of a tile whose rows lie along k: k .. k + 7 from `at` (16-byte aligned)
-  static DEVI u32x4 along(const E *at) { return *reinterpret_cast<const u32x4 *>(at); }
-  // A block of KS rows of pitch P that lie along k: lane i gets column `i` of the 16 whose pieces of 4 lie at
-  // `first + step * (i % 4)` of a row.
-  template <int P> static DEVI u32x4 across(const E *block, int first, int step, int i, int g) {
-    const E *src = block + (8 * g + (i >> 2)) * P + first + step * (i & 3);
-    const frag_i16x4 lo = lds_transposed(src), hi = lds_transposed(src + 4 * P);
+  // A tile in LDS: rows of COLS values without padding, their pieces of 16 bytes permuted within the row.  A read of 16 bytes a lane is
+  // served 16 lanes at a time, and those are i in 0..3, 12..15 of one group g and 4..11 of the next: along the rows they meet in no
+  // bank where four rows' permutations go 0, 3, 2, 1 (0, 1, 2, 3 in order: two by two, 8 cycles an instruction and not 6).
+  template <int COLS> static DEVI int swz(int row) {
+    const int low = -(row >> 2) & 3;
+    return COLS >= 128 ? (row & 3) << 2 | low : (row >> 1 & 1) << 2 | low;
+  }
+  template <int COLS> static DEVI int place(int row, int piece) { return row * COLS + (piece ^ swz<COLS>(row)) * V; }
+  static constexpr int size(int rows, int cols) { return rows * cols * 2; }  // bytes
+  // A lane's places (bytes) in tiles of COLS columns.  Rows and blocks of KS rows are given by where they begin (a multiple of 16
+  // rows), blocks kb of KS columns by their number.
+  template <int COLS> struct Lane {
+    static constexpr int KB = COLS / KS;
+    int row[KB], krow_row[KB], cols[KB][2];
+    DEVI Lane(int i, int g, int half) {
+#pragma unroll
+      for (int kb = 0; kb < KB; ++kb) {
+        row[kb] = 2 * place<COLS>(i, 4 * kb + g);
+        krow_row[kb] = 2 * place<COLS>(krow(i, half), 4 * kb + g);
+#pragma unroll
+        for (int h = 0; h < 2; ++h) cols[kb][h] = 2 * place<COLS>(8 * g + 4 * h + (i >> 2), 4 * kb + (i & 3));
+      }
+    }
+    // row i, or row krow(i, half) with the half that the lane was made with: k = KS kb + V g .. + 7
+    DEVI u32x4 along(const char *at, int kb) const { return *reinterpret_cast<const u32x4 *>(at + row[kb]); }
+    DEVI u32x4 along_krow(const char *at, int kb) const { return *reinterpret_cast<const u32x4 *>(at + krow_row[kb]); }
+    // the rows of a block are k: the columns of kb, for tile `half` of them in the order of krow
+    DEVI u32x4 columns(const char *block, int kb, int half) const { return both(block + cols[kb][0] + 8 * half, block + cols[kb][1] + 8 * half); }
+  };
+  // the same for the columns 16 (n + d) .. in order, n a multiple of the number of tiles d
+  template <int COLS> struct ColumnLane {
+    int cols[2];
+    DEVI ColumnLane(int n, int i, int g) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h) cols[h] = 2 * (place<COLS>(8 * g + 4 * h + (i >> 2), 2 * n + (i >> 1 & 1)) + 4 * (i & 1));
+    }
+    DEVI u32x4 columns(const char *block, int d = 0) const { return both(block + (cols[0] ^ 32 * d), block + (cols[1] ^ 32 * d)); }
+  };
+  static DEVI u32x4 both(const char *rows, const char *rows4) {
+    const frag_i16x4 lo = lds_transposed(reinterpret_cast<const uint16_t *>(rows)), hi = lds_transposed(reinterpret_cast<const uint16_t *>(rows4));
     return __builtin_bit_cast(u32x4, (frag_i16x8)__builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
   }
-  // the 16 columns of tile `half` of a block of 32: in the order of krow, or one after the other
-  template <int P> static DEVI u32x4 columns(const E *block, int col, int half, int i, int g) {
-    return across<P>(block, col + 4 * half, 8, i, g);
-  }
-  template <int P> static DEVI u32x4 columns_in_order(const E *block, int col, int i, int g) { return across<P>(block, col, 4, i, g); }
   static DEVI void gather(const f32x4 (&t)[2], float (&v)[8]) {
 #pragma unroll
     for (int e = 0; e < 4; ++e) v[e] = t[0][e], v[4 + e] = t[1][e];
@@ -90,6 +118,14 @@ template <> struct Frags<bf16_t> : Frags16<bf16_t> {
   static DEVI void unpack(u32x4 w, float (&v)[8]) {
 #pragma unroll
     for (int e = 0; e < 4; ++e) v[2 * e] = bf16_lo(w[e]), v[2 * e + 1] = bf16_hi(w[e]);
+  }
+  // What a lane holds of a tile of results: into row `row` of a tile in LDS, as the columns 16 n + 4 g .. ..
+  template <int COLS> static DEVI void store(char *tile, int row, int n, int g, f32x4 v) {
+    *reinterpret_cast<u32x2 *>(tile + 2 * (place<COLS>(row, 2 * n + (g >> 1)) + 4 * (g & 1))) = u32x2{pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3])};
+  }
+  // .. or as the tile `half` of the lane's computed fragment
+  static DEVI void store_comp(Comp *frag, int half, f32x4 v) {
+    reinterpret_cast<u32x2 *>(frag)[half] = u32x2{pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3])};
   }
   static DEVI u32x4 pack(const float (&v)[8]) {
     return u32x4{pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3]), pack_bf16(v[4], v[5]), pack_bf16(v[6], v[7])};
@@ -109,6 +145,14 @@ template <> struct Frags<f16_t> : Frags16<f16_t> {
   static DEVI void unpack(u32x4 w, float (&v)[8]) {
 #pragma unroll
     for (int e = 0; e < 4; ++e) v[2 * e] = f16_lo(w[e]), v[2 * e + 1] = f16_hi(w[e]);
+  }
+  template <int COLS> static DEVI void store(char *tile, int row, int n, int g, f32x4 v) {
+    *reinterpret_cast<u32x2 *>(tile + 2 * (place<COLS>(row, 2 * n + (g >> 1)) + 4 * (g & 1))) = u32x2{pack_f16(v[0], v[1]), pack_f16(v[2], v[3])};
+  }
+  static DEVI void store_comp(Comp *frag, int half, f32x4 v) {
+    const u32x2 hi = {pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3])};
+    reinterpret_cast<u32x2 *>(&frag->h)[half] = hi;
+    reinterpret_cast<u32x2 *>(&frag->l)[half] = u32x2{pack_bf16(v[0] - bf16_lo(hi[0]), v[1] - bf16_hi(hi[0])), pack_bf16(v[2] - bf16_lo(hi[1]), v[3] - bf16_hi(hi[1]))};
   }
   static DEVI u32x4 pack(const float (&v)[8]) {
     return u32x4{pack_f16(v[0], v[1]), pack_f16(v[2], v[3]), pack_f16(v[4], v[5]), pack_f16(v[6], v[7])};
@@ -134,16 +178,29 @@ template <> struct Frags<float> {
   using Data = Frag32;
   using Comp = Frag32;
   using Wide = Frag32;
-  static constexpr int KS = 16, NT = 1, V = 4, PAD = 4;
+  static constexpr int KS = 16, NT = 1, V = 4;
   static DEVI int krow(int m, int) { return m; }
-  static DEVI f32x4 along(const E *at) { return *reinterpret_cast<const f32x4 *>(at); }
-  template <int P> static DEVI f32x4 columns_in_order(const E *block, int col, int i, int g) {
-    f32x4 v;
+  // (columns are read element by element here: 4 elements of padding a row keep them and the rows apart)
+  template <int COLS> static DEVI int place(int row, int piece) { return row * (COLS + 4) + piece * V; }
+  static constexpr int size(int rows, int cols) { return rows * (cols + 4) * 4; }  // bytes
+  template <int COLS> struct ColumnLane {
+    int col;
+    DEVI ColumnLane(int n, int i, int g) { col = 4 * (4 * g * (COLS + 4) + 16 * n + i); }
+    DEVI f32x4 columns(const char *block, int d = 0) const {
+      f32x4 v;
 #pragma unroll
-    for (int r = 0; r < 4; ++r) v[r] = block[(4 * g + r) * P + col + i];
-    return v;
-  }
-  template <int P> static DEVI f32x4 columns(const E *block, int col, int, int i, int g) { return columns_in_order<P>(block, col, i, g); }
+      for (int r = 0; r < 4; ++r) v[r] = *reinterpret_cast<const float *>(block + col + 4 * (r * (COLS + 4) + 16 * d));
+      return v;
+    }
+  };
+  template <int COLS> struct Lane {
+    int row;
+    ColumnLane<COLS> cols;
+    DEVI Lane(int i, int g, int) : cols(0, i, g) { row = 4 * (i * (COLS + 4) + V * g); }
+    DEVI f32x4 along(const char *at, int kb) const { return *reinterpret_cast<const f32x4 *>(at + row + 4 * KS * kb); }
+    DEVI f32x4 along_krow(const char *at, int kb) const { return along(at, kb); }
+    DEVI f32x4 columns(const char *block, int kb, int) const { return cols.columns(block + 4 * KS * kb); }
+  };
   static DEVI void gather(const f32x4 (&t)[1], float (&v)[4]) {
 #pragma unroll
     for (int e = 0; e < 4; ++e) v[e] = t[0][e];
@@ -154,6 +211,8 @@ template <> struct Frags<float> {
 #pragma unroll
     for (int e = 0; e < 4; ++e) v[e] = w[e];
   }
+  template <int COLS> static DEVI void store(char *tile, int row, int n, int g, f32x4 v) { *reinterpret_cast<f32x4 *>(tile + 4 * place<COLS>(row, 4 * n + g)) = v; }
+  static DEVI void store_comp(Comp *frag, int, f32x4 v) { frag->v = v; }
   static DEVI f32x4 pack(const float (&v)[4]) { return f32x4{v[0], v[1], v[2], v[3]}; }
   static DEVI Frag32 comp(const float (&v)[4]) { return Frag32{f32x4{v[0], v[1], v[2], v[3]}}; }
   static DEVI Frag32 wide(const float (&v)[4]) { return comp(v); }

@@ -45,8 +45,10 @@ template <typename T, int D, bool RAG> __global__ __launch_bounds__(kThreads) vo
   using F = Frags<T>;
   using E = typename F::E;
   using Raw = typename F::Raw;
-  constexpr int KS = F::KS, NT = F::NT, V = F::V, KB = D / KS, OT = D / 16, PER = D / V, NV = KS * PER / 64, PITCH = D + F::PAD;
-  constexpr int AREA = KS * PITCH * (int)sizeof(E) > kHeads * (D + 4) * 4 ? KS * PITCH * (int)sizeof(E) : kHeads * (D + 4) * 4;
+  using Columns = typename F::template ColumnLane<D>;
+  constexpr int KS = F::KS, NT = F::NT, V = F::V, KB = D / KS, OT = D / 16, PER = D / V, NV = KS * PER / 64;
+  constexpr int AREA = kHeads * (D + 4) * 4;
+  static_assert(F::size(KS, D) <= AREA, "a tile of values");
   __shared__ __align__(16) char area[kWaves][AREA];
   __shared__ float wave_m[kWaves][kHeads], wave_l[kWaves][kHeads];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), i = lane & 15, g = lane >> 4;
@@ -168,7 +170,7 @@ template <typename T, int D, bool RAG> __global__ __launch_bounds__(kThreads) vo
 #pragma unroll
     for (int n = 0; n < NV; ++n) {
       const int id = n * 64 + lane;
-      *reinterpret_cast<Raw *>(tile_v + id / PER * PITCH + id % PER * V) = vr[n];
+      *reinterpret_cast<Raw *>(tile_v + F::template place<D>(id / PER, id % PER)) = vr[n];
     }
     if (more) load_v(next);
     if (now.mask) {
@@ -195,7 +197,7 @@ template <typename T, int D, bool RAG> __global__ __launch_bounds__(kThreads) vo
 #pragma unroll
       for (int d = 0; d < OT; ++d) {
         o[d] *= shrink;
-        o[d] = F::mma_raw(F::template columns_in_order<PITCH>(tile_v, 16 * d, i, g), pf, o[d]);
+        o[d] = F::mma_raw(Columns(d, i, g).columns(area[wave]), pf, o[d]);
       }
     }
     now = next;
