@@ -10,8 +10,8 @@ using namespace lin;
 template <typename T, int KD, int DVT, Fit FIT> __global__ __launch_bounds__(kThreads, (Shape<T, KD, DVT>::WORKGROUPS)) void lin_segment_kernel(const LinLaunch p) {
   using F = Frags<T>;
   using Sh = Shape<T, KD, DVT>;
-  constexpr int C = Sh::C;
-  __shared__ __align__(16) char lds[2][Sh::STAGE];  // (the rows a stay out)
+  constexpr int C = Sh::C, TURN = 2 * C, CC = F::size(TURN, KD);  // two blocks a barrier: more rows on their way
+  __shared__ __align__(16) char lds[2][CC + F::size(TURN, Sh::VAL)];
   const Place at = place_of(p);
   if (at.none) return;
   const LinWalk &w = p.w[at.walk];
@@ -25,52 +25,56 @@ template <typename T, int KD, int DVT, Fit FIT> __global__ __launch_bounds__(kTh
   int64_t b_ls, c_ls;
   const T *b = static_cast<const T *>(w.b.p) + rows_at(w.b, it, at.head, w.reverse, p.seg_len, b_ls);
   const T *c = static_cast<const T *>(w.c.p) + rows_at(w.c, it, at.head, w.reverse, p.seg_len, c_ls) + v0;
-  Stage<T, C, KD, FIT> sb(b, b_ls, w.key, tid);
-  Stage<T, C, Sh::VAL, FIT> sc(c, c_ls, min(w.val - v0, Sh::VAL), tid);
+  Stage<T, TURN, KD, FIT> sb(b, b_ls, w.key, tid);
+  Stage<T, TURN, Sh::VAL, FIT> sc(c, c_ls, min(w.val - v0, Sh::VAL), tid);
   WaveState<T, KD, DVT> state;
   state.zero();
   const float write = w.write;
   const int late = w.late;
   const Weights<F, Sh::JB, Sh::IT> weights(decay, 0.f, write, late, i, g);
   auto fetch = [&](int t) {
-    const int n = min(it.n - t, C);
+    const int n = min(it.n - t, TURN);
     sb.fetch(b + t * b_ls, b_ls, n, tid), sc.fetch(c + t * c_ls, c_ls, n, tid);
   };
   auto commit = [&](auto whole, int t, char *rows) {
-    const int n = min(it.n - t, C);
-    sb.template commit<whole.value>(rows + Sh::B, n, tid), sc.template commit<whole.value>(rows + Sh::CC, n, tid);
+    const int n = min(it.n - t, TURN);
+    sb.template commit<whole.value>(rows, n, tid), sc.template commit<whole.value>(rows + CC, n, tid);
   };
-  // whole: so are this block and the next two
-  auto block = [&](auto whole, int t, char *now, char *next) {
+  // whole: so are these two blocks and the next four
+  auto turn = [&](auto whole, int t, char *now, char *next) {
     constexpr bool FULL = whole.value;
-    if (FULL || t + C < it.n) commit(whole, t + C, next);
+    if (FULL || t + TURN < it.n) commit(whole, t + TURN, next);
     if constexpr (FULL) sb.fetch_next(), sc.fetch_next();
-    else if (t + 2 * C < it.n) fetch(t + 2 * C);
-    state.template update<FULL>(now, lanes, values, decay, weights, write, FULL ? C : min(it.n - t, C), late, g);
+    else if (t + 2 * TURN < it.n) fetch(t + 2 * TURN);
+#pragma unroll
+    for (int k = 0; k < 2; ++k)
+      if (FULL || t + k * C < it.n)
+        state.template update<FULL>(now + F::size(k * C, KD), now + CC + F::size(k * C, Sh::VAL), lanes, values, decay, weights, write,
+                                    FULL ? C : min(it.n - t - k * C, C), late, g);
     lds_barrier();
   };
   char *now = lds[0], *next = lds[1];
-  const bool steady = FIT != ELEMENTS && it.n >= 3 * C && near(w.b) && near(w.c);
+  const bool steady = FIT != ELEMENTS && it.n >= 3 * TURN && near(w.b) && near(w.c);
   int t = 0;
   if (steady) {
     sb.fetch_next(), sc.fetch_next();
     commit(std::true_type{}, 0, now);
     sb.fetch_next(), sc.fetch_next();
     lds_barrier();
-    for (; t + 3 * C <= it.n; t += C) {
-      block(std::true_type{}, t, now, next);
+    for (; t + 3 * TURN <= it.n; t += TURN) {
+      turn(std::true_type{}, t, now, next);
       char *const was = now;
       now = next, next = was;
     }
   } else {
     fetch(0);
     commit(std::false_type{}, 0, now);
-    if (C < it.n) fetch(C);
+    if (TURN < it.n) fetch(TURN);
     lds_barrier();
   }
 #pragma unroll 1
-  for (; t < it.n; t += C) {
-    block(std::false_type{}, t, now, next);
+  for (; t < it.n; t += TURN) {
+    turn(std::false_type{}, t, now, next);
     char *const was = now;
     now = next, next = was;
   }
@@ -283,7 +287,7 @@ template <typename T, int KD, int DVT, Fit FIT, bool PARTS> __global__ __launch_
         }
       }
     }
-    state.template update<FULL>(now, lanes, values, decay, weights, write, n, late, g);
+    state.template update<FULL>(now + Sh::B, now + Sh::CC, lanes, values, decay, weights, write, n, late, g);
     if (FULL || t + C < it.n) scores(next, s_next);
     lds_barrier();
   };

@@ -268,9 +268,9 @@ template <typename T, int KD, int DVT> struct WaveState {
             t[d][kb][h][r] = f(t[d][kb][h][r], d, k, k < key);
           }
   }
-  // f^n Z + write b^T diag(f^(n - late - s)) c over the n positions of a stage's rows
+  // f^n Z + write b^T diag(f^(n - late - s)) c over the n positions of a block's rows
   template <bool FULL, typename WT>
-  DEVI void update(const char *rows, const typename F::template Lane<KD> &lanes, const Values &values, const Decay &f, const WT &weights, float write, int n, int late,
+  DEVI void update(const char *b_rows, const char *c_rows, const typename F::template Lane<KD> &lanes, const Values &values, const Decay &f, const WT &weights, float write, int n, int late,
                    int g) {
     constexpr int V = F::V;
     const float keep = FULL ? weights.keep : f(n);
@@ -281,7 +281,7 @@ template <typename T, int KD, int DVT> struct WaveState {
 #pragma unroll
       for (int d = 0; d < DVT; ++d) {
         float v[V];
-        F::unpack(values.columns(rows + Sh::CC + F::size(F::KS * jb, Sh::VAL), d), v);
+        F::unpack(values.columns(c_rows + F::size(F::KS * jb, Sh::VAL), d), v);
         if constexpr (FULL) {
           const float lane = weights.up_lane * weights.up_block[jb];
 #pragma unroll
@@ -296,7 +296,7 @@ template <typename T, int KD, int DVT> struct WaveState {
       for (int kb = 0; kb < Sh::KB; ++kb)
 #pragma unroll
         for (int h = 0; h < F::NT; ++h) {
-          const typename F::Data b = F::data(lanes.columns(rows + Sh::B + F::size(F::KS * jb, KD), kb, h));
+          const typename F::Data b = F::data(lanes.columns(b_rows + F::size(F::KS * jb, KD), kb, h));
 #pragma unroll
           for (int d = 0; d < DVT; ++d) t[d][kb][h] = mma16(b, wc[d], t[d][kb][h]);
         }
