@@ -6,10 +6,16 @@
 namespace {
 using namespace lin;
 
+// EXACT: a state is a result, in fp32, and the weighted rows that are added to it are split into three bf16 parts, 2^-25 of a value.  Else
+// two, 2^-17, are more than results of 16 bits show (8 x 4096 x 20 x 128 in bf16, forward and backward: 671 us of kernels with two,
+// 764 with three; 726 with both in one kernel).
+template <typename F, bool EXACT> using Parts = std::conditional_t<EXACT, typename F::Wider, typename F::Wide>;
+
 // The state of one segment alone, from zero, for the segments behind it.
-template <typename T, int KD, int DVT, Fit FIT> __global__ __launch_bounds__(kThreads, (Shape<T, KD, DVT>::WORKGROUPS)) void lin_segment_kernel(const LinLaunch p) {
+template <typename T, int KD, int DVT, Fit FIT, bool EXACT> __global__ __launch_bounds__(kThreads, (Shape<T, KD, DVT>::WORKGROUPS)) void lin_segment_kernel(const LinLaunch p) {
   using F = Frags<T>;
   using Sh = Shape<T, KD, DVT>;
+  using W = Parts<F, EXACT>;
   constexpr int C = Sh::C, TURN = 2 * C, CC = F::size(TURN, KD);  // two blocks a barrier: more rows on their way
   __shared__ __align__(16) char lds[2][CC + F::size(TURN, Sh::VAL)];
   const Place at = place_of(p);
@@ -49,7 +55,7 @@ template <typename T, int KD, int DVT, Fit FIT> __global__ __launch_bounds__(kTh
 #pragma unroll
     for (int k = 0; k < 2; ++k)
       if (FULL || t + k * C < it.n)
-        state.template update<FULL>(now + F::size(k * C, KD), now + CC + F::size(k * C, Sh::VAL), lanes, values, decay, weights, write,
+        state.template update<FULL, W>(now + F::size(k * C, KD), now + CC + F::size(k * C, Sh::VAL), lanes, values, decay, weights, write,
                                     FULL ? C : min(it.n - t - k * C, C), late, g);
     lds_barrier();
   };
@@ -85,9 +91,10 @@ template <typename T, int KD, int DVT, Fit FIT> __global__ __launch_bounds__(kTh
 
 // PARTS: there are walks whose y is a part of a sum, in fp32.  (The loop for those beside the other one costs registers that the
 // launches without them need: 8 spilled a block.)
-template <typename T, int KD, int DVT, Fit FIT, bool PARTS> __global__ __launch_bounds__(kThreads, (Shape<T, KD, DVT>::WORKGROUPS)) void lin_walk_kernel(const LinLaunch p) {
+template <typename T, int KD, int DVT, Fit FIT, bool PARTS, bool EXACT> __global__ __launch_bounds__(kThreads, (Shape<T, KD, DVT>::WORKGROUPS)) void lin_walk_kernel(const LinLaunch p) {
   using F = Frags<T>;
   using Sh = Shape<T, KD, DVT>;
+  using W = Parts<F, EXACT>;
   using Raw = typename F::Raw;
   constexpr int C = Sh::C, KB = Sh::KB, JB = Sh::JB, IT = Sh::IT, NT = F::NT, KS = F::KS, V = F::V;
   __shared__ __align__(16) char lds[Sh::LDS];
@@ -287,7 +294,7 @@ template <typename T, int KD, int DVT, Fit FIT, bool PARTS> __global__ __launch_
         }
       }
     }
-    state.template update<FULL>(now + Sh::B, now + Sh::CC, lanes, values, decay, weights, write, n, late, g);
+    state.template update<FULL, W>(now + Sh::B, now + Sh::CC, lanes, values, decay, weights, write, n, late, g);
     if (FULL || t + C < it.n) scores(next, s_next);
     lds_barrier();
   };
@@ -461,21 +468,23 @@ Cut cut_of(const LinearAttnParams &p, int nwalks) {
   return c;
 }
 
-template <typename T, int KD, int DVT, Fit FIT> int run(const LinLaunch &l, hipStream_t st) {
+template <typename T, int KD, int DVT, Fit FIT, bool PARTS, bool EXACT> int launch(const LinLaunch &l, hipStream_t st) {
   const int64_t outer = ((int64_t)l.items * l.kv_heads + 7) / 8 * 8, blocks = outer * (l.nheads / l.kv_heads) * l.nwalks * l.slices;
   if (blocks > INT32_MAX) return MAMBA_E_UNSUPPORTED;
   if (l.nseg > 1) {
-    lin_segment_kernel<T, KD, DVT, FIT><<<(int)blocks, kThreads, 0, st>>>(l);
+    lin_segment_kernel<T, KD, DVT, FIT, EXACT><<<(int)blocks, kThreads, 0, st>>>(l);
     if (hipGetLastError() != hipSuccess) return MAMBA_E_LAUNCH;
   }
-  if constexpr (sizeof(T) < 4) {
-    if (l.w[l.nwalks - 1].y_f32) {
-      lin_walk_kernel<T, KD, DVT, FIT, true><<<(int)blocks, kThreads, 0, st>>>(l);
-      return hipGetLastError() == hipSuccess ? MAMBA_OK : MAMBA_E_LAUNCH;
-    }
-  }
-  lin_walk_kernel<T, KD, DVT, FIT, false><<<(int)blocks, kThreads, 0, st>>>(l);
+  lin_walk_kernel<T, KD, DVT, FIT, PARTS, EXACT><<<(int)blocks, kThreads, 0, st>>>(l);
   return hipGetLastError() == hipSuccess ? MAMBA_OK : MAMBA_E_LAUNCH;
+}
+template <typename T, int KD, int DVT, Fit FIT> int run(const LinLaunch &l, hipStream_t st) {
+  if constexpr (sizeof(T) < 4) {
+    const LinWalk &last = l.w[l.nwalks - 1];  // the walk of the values: its state is the result, and heads that share are its sums too
+    if (last.y_f32) return launch<T, KD, DVT, FIT, true, true>(l, st);
+    if (last.end.p) return launch<T, KD, DVT, FIT, false, true>(l, st);
+  }
+  return launch<T, KD, DVT, FIT, false, false>(l, st);
 }
 template <typename T, int KD, int DVT> int run_fit(const LinLaunch &l, const Cut &c, hipStream_t st) {
   switch (c.fit) {

@@ -268,16 +268,16 @@ template <typename T, int KD, int DVT> struct WaveState {
             t[d][kb][h][r] = f(t[d][kb][h][r], d, k, k < key);
           }
   }
-  // f^n Z + write b^T diag(f^(n - late - s)) c over the n positions of a block's rows
-  template <bool FULL, typename WT>
-  DEVI void update(const char *b_rows, const char *c_rows, const typename F::template Lane<KD> &lanes, const Values &values, const Decay &f, const WT &weights, float write, int n, int late,
-                   int g) {
+  // f^n Z + write b^T diag(f^(n - late - s)) c over the n positions of a block's rows, the weighted c in two parts or three (W)
+  template <bool FULL, typename W, typename WT>
+  DEVI void update(const char *b_rows, const char *c_rows, const typename F::template Lane<KD> &lanes, const Values &values, const Decay &f, const WT &weights,
+                   float write, int n, int late, int g) {
     constexpr int V = F::V;
     const float keep = FULL ? weights.keep : f(n);
     each([&](f32x4 &v, int) { v *= keep; });
 #pragma unroll
     for (int jb = 0; jb < Sh::JB; ++jb) {
-      typename F::Wide wc[DVT];
+      W wc[DVT];
 #pragma unroll
       for (int d = 0; d < DVT; ++d) {
         float v[V];
@@ -290,7 +290,7 @@ template <typename T, int KD, int DVT> struct WaveState {
 #pragma unroll
           for (int e = 0; e < V; ++e) v[e] *= write * f(max(n - late - (F::KS * jb + V * g + e), 0));
         }
-        wc[d] = F::wide(v);
+        wc[d] = F::template wide<W>(v);
       }
 #pragma unroll
       for (int kb = 0; kb < Sh::KB; ++kb)

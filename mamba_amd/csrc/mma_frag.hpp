@@ -8,8 +8,8 @@
 //   bf16: one instruction for 32 k.  fp16: data times data as it is (exact); where one side has been computed (a weighted
 //   sum leaves fp16's range at 65504) both sides are split into two bf16 parts, 16 bits together, three instructions.
 //   fp32: four instructions of 4 k, products and sums in fp32.
-// Data: fragments that hold operands as they lie in memory.  Wide: a computed one in two parts.  Comp: a computed one in as
-// many parts as the result's type can show.
+// Data: fragments that hold operands as they lie in memory.  Comp: a computed one in as many parts as the result's type can show.
+// Wide, Wider: in two bf16 parts, 16 bits together, and in three, 24 bits.
 #pragma once
 #include "common.hpp"
 
@@ -38,6 +38,24 @@ struct Split {
 DEVI f32x4 mma16(const Split &a, const Split &b, f32x4 c) { return mma16(a.h, b.h, mma16(a.h, b.l, mma16(a.l, b.h, c))); }
 DEVI f32x4 mma16(const Split &a, frag_bf16x8 b, f32x4 c) { return mma16(a.h, b, mma16(a.l, b, c)); }
 DEVI f32x4 mma16(frag_bf16x8 a, const Split &b, f32x4 c) { return mma16(a, b.h, mma16(a, b.l, c)); }
+
+// three bf16 parts: 24 bits
+struct Split3 {
+  frag_bf16x8 h, m, l;
+  DEVI void set(const float (&v)[8]) {
+    u32x4 hi, mid, lo;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      hi[e] = pack_bf16(v[2 * e], v[2 * e + 1]);
+      const float a = v[2 * e] - bf16_lo(hi[e]), b = v[2 * e + 1] - bf16_hi(hi[e]);
+      mid[e] = pack_bf16(a, b);
+      lo[e] = pack_bf16(a - bf16_lo(mid[e]), b - bf16_hi(mid[e]));
+    }
+    h = __builtin_bit_cast(frag_bf16x8, hi), m = __builtin_bit_cast(frag_bf16x8, mid), l = __builtin_bit_cast(frag_bf16x8, lo);
+  }
+};
+DEVI f32x4 mma16(frag_bf16x8 a, const Split3 &b, f32x4 c) { return mma16(a, b.h, mma16(a, b.m, mma16(a, b.l, c))); }
+DEVI f32x4 mma16(const Split &a, const Split3 &b, f32x4 c) { return mma16(a.h, b.h, mma16(a.l, b.h, mma16(a.h, b.m, mma16(a.l, b.m, mma16(a.h, b.l, c))))); }
 
 struct Frag32 {
   f32x4 v;
@@ -113,6 +131,7 @@ template <> struct Frags<bf16_t> : Frags16<bf16_t> {
   using Data = frag_bf16x8;
   using Comp = frag_bf16x8;
   using Wide = Split;
+  using Wider = Split3;
   static DEVI Data data(u32x4 w) { return __builtin_bit_cast(frag_bf16x8, w); }
   static DEVI f32x4 mma_raw(u32x4 a, u32x4 b, f32x4 c) { return mma16(data(a), data(b), c); }
   static DEVI void unpack(u32x4 w, float (&v)[8]) {
@@ -131,8 +150,8 @@ template <> struct Frags<bf16_t> : Frags16<bf16_t> {
     return u32x4{pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3]), pack_bf16(v[4], v[5]), pack_bf16(v[6], v[7])};
   }
   static DEVI Comp comp(const float (&v)[8]) { return data(pack(v)); }
-  static DEVI Wide wide(const float (&v)[8]) {
-    Split s;
+  template <typename W> static DEVI W wide(const float (&v)[8]) {
+    W s;
     s.set(v);
     return s;
   }
@@ -142,6 +161,7 @@ template <> struct Frags<f16_t> : Frags16<f16_t> {
   using Data = Split;
   using Comp = Split;
   using Wide = Split;
+  using Wider = Split3;
   static DEVI void unpack(u32x4 w, float (&v)[8]) {
 #pragma unroll
     for (int e = 0; e < 4; ++e) v[2 * e] = f16_lo(w[e]), v[2 * e + 1] = f16_hi(w[e]);
@@ -160,17 +180,21 @@ template <> struct Frags<f16_t> : Frags16<f16_t> {
   static DEVI Data data(u32x4 w) {
     float v[8];
     unpack(w, v);
-    return wide(v);
+    return comp(v);
   }
   static DEVI f32x4 mma_raw(u32x4 a, u32x4 b, f32x4 c) {
     return mma16(__builtin_bit_cast(frag_f16x8, a), __builtin_bit_cast(frag_f16x8, b), c);
   }
-  static DEVI Split wide(const float (&v)[8]) {
+  template <typename W> static DEVI W wide(const float (&v)[8]) {
+    W s;
+    s.set(v);
+    return s;
+  }
+  static DEVI Comp comp(const float (&v)[8]) {
     Split s;
     s.set(v);
     return s;
   }
-  static DEVI Comp comp(const float (&v)[8]) { return wide(v); }
 };
 template <> struct Frags<float> {
   using E = float;
@@ -178,6 +202,7 @@ template <> struct Frags<float> {
   using Data = Frag32;
   using Comp = Frag32;
   using Wide = Frag32;
+  using Wider = Frag32;
   static constexpr int KS = 16, NT = 1, V = 4;
   static DEVI int krow(int m, int) { return m; }
   // (columns are read element by element here: 4 elements of padding a row keep them and the rows apart)
@@ -215,5 +240,5 @@ template <> struct Frags<float> {
   static DEVI void store_comp(Comp *frag, int, f32x4 v) { frag->v = v; }
   static DEVI f32x4 pack(const float (&v)[4]) { return f32x4{v[0], v[1], v[2], v[3]}; }
   static DEVI Frag32 comp(const float (&v)[4]) { return Frag32{f32x4{v[0], v[1], v[2], v[3]}}; }
-  static DEVI Frag32 wide(const float (&v)[4]) { return comp(v); }
+  template <typename W> static DEVI W wide(const float (&v)[4]) { return comp(v); }
 };
