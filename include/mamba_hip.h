@@ -892,7 +892,8 @@ int linear_attn_state_update(const LinearAttnStepParams *p, mamba_stream_t strea
  * A negative cache_seqlens[b] is a padding entry: nothing is written, out is 0; so it is where no position counts.  A length
  * beyond max_pages * page_size counts as that.  Pages outside of [0, num_pages) have no positions: they are left out, and a token
  * whose page is one takes part without being written.
- * nsplit parts of the cache's length are worked on side by side (paged_attn_parts says how many suit; 1: no workspace);
+ * nsplit: even ranges of all sequences' positions that are worked on side by side, up to 512 (paged_attn_parts says how many suit; 1:
+ * a workgroup per sequence and key head, no workspace);
  * ws: paged_attn_ws_bytes of 16-byte aligned memory, contents ignored on entry.  Head sizes up to 256, max_pages * page_size up to
  * 2^30, batch up to 65535.
  * ------------------------------------------------------------------------- */
