@@ -57,6 +57,9 @@ template <typename T, int D, bool RAG> __global__ __launch_bounds__(kThreads, RA
   constexpr int LD = D == 96 ? 128 : D;  // columns of a tile in LDS, whose rows are permuted by powers of two
   using Columns = typename F::template ColumnLane<LD>;
   constexpr int KS = F::KS, NT = F::NT, V = F::V, KB = D / KS, OT = D / 16, PER = D / V, NV = KS * PER / 64;
+  // l and o are kLift times the sums: weights of 2^-29 of the largest are still whole fp16 numbers, and the last ones left out are below
+  // 2^-40 (without it below 2^-25, which many positions beside one that draws the weight add up to a result).
+  constexpr float kLift = std::is_same_v<T, f16_t> ? 32768.f : 1.f;
   constexpr int TILE = F::size(KS, LD), SUMS = kHeads * (D + 4) * 4, AREA = TILE > SUMS ? TILE : SUMS;
   __shared__ __align__(16) char area[kWaves][AREA];
   __shared__ float wave_m[kWaves][kHeads], wave_l[kWaves][kHeads];
@@ -252,10 +255,10 @@ template <typename T, int D, bool RAG> __global__ __launch_bounds__(kThreads, RA
       l *= shrink;
 #pragma unroll
       for (int e = 0; e < V; ++e) {
-        v[e] = fast_exp2(v[e] - m);
+        v[e] = fast_exp2(v[e] - m) * kLift;
         l += v[e];
       }
-      const Raw pf = F::pack(v);  // 0 .. 1: the type's own format holds them; l has them unrounded
+      const Raw pf = F::pack(v);  // 0 .. kLift: the type's own format holds them; l has them unrounded
 #pragma unroll
       for (int d = 0; d < OT; ++d) {
         o[d] *= shrink;
