@@ -835,6 +835,8 @@ int norm_block_bwd_nparts(const NormBlockParams *p);
  * sequence count for nothing: their outputs and gradients are 0.
  * Head sizes up to 256, seqlen up to 2^30.  ws: linear_attn_fwd_ws_bytes / linear_attn_bwd_ws_bytes of 16-byte aligned memory
  * (0: none), contents ignored on entry, nothing in it is kept between calls.  Every result repeats bit for bit.
+ * No result shares memory with an operand, with another result or with ws: workgroups write while others still read.  States that
+ * meet (final_states with initial_states, dinitial_states with either) and rows that begin where an operand's do are MAMBA_E_BADARG.
  * ------------------------------------------------------------------------- */
 typedef struct LinearAttnParams {
   int32_t batch, seqlen, nheads, nkvheads, headdim_k, headdim_v;
@@ -866,7 +868,7 @@ int linear_attn_bwd(const LinearAttnParams *p, mamba_stream_t stream);
 /* One position of the same recurrence: state (state_rows, nheads, headdim_k, headdim_v), each row dense, is updated in place,
  * out (batch, nheads, headdim_v) is scale q S of the new state.  Row state_batch_indices[b] of the state belongs to entry b (row b
  * without them); an index outside [0, state_rows) is a padding entry: no state is touched, out is 0.  The rows named have to be
- * different ones.  Up to 65535 heads. */
+ * different ones.  out shares memory with no operand.  Up to 65535 heads. */
 typedef struct LinearAttnStepParams {
   int32_t batch, nheads, nkvheads, headdim_k, headdim_v, state_rows;
   int32_t dtype, state_dtype;
@@ -894,8 +896,9 @@ int linear_attn_state_update(const LinearAttnStepParams *p, mamba_stream_t strea
  * whose page is one takes part without being written.
  * nsplit: even ranges of all sequences' positions that are worked on side by side, up to 512 (paged_attn_parts says how many suit; 1:
  * a workgroup per sequence and key head, no workspace);
- * ws: paged_attn_ws_bytes of 16-byte aligned memory, contents ignored on entry.  Head sizes up to 256, max_pages * page_size up to
- * 2^30, batch up to 65535.
+ * ws: paged_attn_ws_bytes of 16-byte aligned memory, contents ignored on entry.  out shares memory with none of k, v and the caches,
+ * and where a token is written no element of one cache is one of the other.  Head sizes up to 256, max_pages * page_size up to 2^30,
+ * batch up to 65535.
  * ------------------------------------------------------------------------- */
 typedef struct PagedAttnParams {
   int32_t batch, nheads, nkvheads, headdim_k, headdim_v;

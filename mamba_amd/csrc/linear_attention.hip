@@ -2,6 +2,7 @@
 #include "linear_attn.hpp"
 
 #include <algorithm>
+#include <initializer_list>
 
 namespace {
 using namespace lin;
@@ -528,6 +529,13 @@ int check(const LinearAttnParams *p) {
   if (p->headdim_k > 256 || p->headdim_v > 256 || p->seqlen > 1 << 30 || p->nseq > 1 << 30) return MAMBA_E_UNSUPPORTED;
   return MAMBA_OK;
 }
+// Workgroups write results while others still read: states that meet, or rows that begin where an operand's do, are refused.
+bool apart(const LinearAttnParams &p, const float *a, const float *b) {
+  const int64_t states = (int64_t)(p.nseq > 0 ? p.nseq : p.batch) * p.nheads * p.headdim_k * p.headdim_v * 4;
+  const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
+  return !a || !b || (x < y ? y - x : x - y) >= (uint64_t)states;
+}
+bool none_of(const void *result, std::initializer_list<const void *> others) { return std::find(others.begin(), others.end(), result) == others.end(); }
 LinRows rows(const void *t, int64_t bs, int64_t ls, int64_t hs, int group) { return LinRows{const_cast<void *>(t), bs, ls, hs, group}; }
 // a buffer of a call: the plan, the segments' states, fp32 gradients of shared heads
 int64_t parts_bytes(const LinearAttnParams &p) {
@@ -580,6 +588,7 @@ extern "C" int linear_attn_fwd(const LinearAttnParams *p, mamba_stream_t stream)
   if (!p->out) return MAMBA_E_BADARG;
   const Cut c = cut_of(*p, 1);
   if (c.plan_bytes + c.state_bytes > 0 && (!p->ws || reinterpret_cast<uintptr_t>(p->ws) % 16 != 0)) return MAMBA_E_BADARG;
+  if (!apart(*p, p->final_states, p->initial_states) || !none_of(p->out, {p->q, p->k, p->v})) return MAMBA_E_BADARG;
   hipStream_t st = static_cast<hipStream_t>(stream);
   const int group = p->nheads / p->nkvheads;
   LinLaunch l = launch_of(*p, c, 1);
@@ -597,6 +606,10 @@ extern "C" int linear_attn_bwd(const LinearAttnParams *p, mamba_stream_t stream)
   if (!p->dout || !p->dq || !p->dk || !p->dv) return MAMBA_E_BADARG;
   const Cut c = cut_of(*p, 3);
   if (linear_attn_bwd_ws_bytes(p) > 0 && (!p->ws || reinterpret_cast<uintptr_t>(p->ws) % 16 != 0)) return MAMBA_E_BADARG;
+  if (!apart(*p, p->dinitial_states, p->initial_states) || !apart(*p, p->dinitial_states, p->dfinal_states)) return MAMBA_E_BADARG;
+  for (const void *result : {p->dq, p->dk, p->dv})
+    if (!none_of(result, {p->q, p->k, p->v, p->dout})) return MAMBA_E_BADARG;
+  if (p->dq == p->dk || p->dq == p->dv || p->dk == p->dv) return MAMBA_E_BADARG;
   hipStream_t st = static_cast<hipStream_t>(stream);
   const int group = p->nheads / p->nkvheads, dk = p->headdim_k, dv = p->headdim_v;
   LinLaunch l = launch_of(*p, c, 3);

@@ -143,6 +143,8 @@ extern "C" int linear_attn_state_update(const LinearAttnStepParams *p, mamba_str
   if (!p->state_batch_indices && p->state_rows < p->batch) return MAMBA_E_BADARG;
   if (!(p->scale >= -3.4e38f && p->scale <= 3.4e38f)) return MAMBA_E_BADARG;
   if (p->headdim_k > 256 || p->headdim_v > 256 || p->nheads > 65535) return MAMBA_E_UNSUPPORTED;
+  // written by one workgroup while another still reads
+  if (p->out == p->q || p->out == p->k || p->out == p->v || p->out == p->state) return MAMBA_E_BADARG;
   hipStream_t st = static_cast<hipStream_t>(stream);
   switch (p->dtype) {
     case MAMBA_F32: return run_state<float>(*p, st);

@@ -373,7 +373,7 @@ int rows_of_batch(const PagedAttnParams &p) { return p.nkvheads * ((p.nheads / p
 template <typename T, int D> int run(const PagedAttnParams &p, hipStream_t st) {
   constexpr int V = Frags<T>::V;
   const int64_t n = p.nsplit == 1 ? p.batch : p.nsplit, grid = rows_of_batch(p) * (n >= 8 ? (n + 7) / 8 * 8 : n);
-  if (grid > INT32_MAX || p.batch > 65535) return MAMBA_E_UNSUPPORTED;
+  if (grid > INT32_MAX) return MAMBA_E_UNSUPPORTED;
   if (p.headdim_k % V == 0 && p.headdim_v % V == 0) paged_part_kernel<T, D, false><<<(int)grid, kThreads, 0, st>>>(p);
   else paged_part_kernel<T, D, true><<<(int)grid, kThreads, 0, st>>>(p);
   if (hipGetLastError() != hipSuccess) return MAMBA_E_LAUNCH;
@@ -423,6 +423,8 @@ extern "C" int paged_attn_update(const PagedAttnParams *p, mamba_stream_t stream
   if (!p->q || !p->k_cache || !p->v_cache || !p->block_table || !p->cache_seqlens || !p->out || (p->k == nullptr) != (p->v == nullptr))
     return MAMBA_E_BADARG;
   if (p->nsplit <= 0 || p->nsplit > kMostParts || (p->nsplit > 1 && (!p->ws || reinterpret_cast<uintptr_t>(p->ws) % 16 != 0))) return MAMBA_E_BADARG;
+  if (p->batch > 65535) return MAMBA_E_UNSUPPORTED;
+  if (p->out == p->k || p->out == p->v || p->out == p->k_cache || p->out == p->v_cache) return MAMBA_E_BADARG;  // (others still read them)
   hipStream_t st = static_cast<hipStream_t>(stream);
   switch (p->dtype) {
     case MAMBA_F32: return run_size<float>(*p, st);
