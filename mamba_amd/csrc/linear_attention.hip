@@ -477,12 +477,13 @@ Cut cut_of(const LinearAttnParams &p, int nwalks) {
 
 template <typename T, int KD, int DVT, Fit FIT, bool PARTS, bool EXACT> int launch(const LinLaunch &l, hipStream_t st) {
   const int64_t outer = ((int64_t)l.items * l.kv_heads + 7) / 8 * 8, blocks = outer * (l.nheads / l.kv_heads) * l.nwalks * l.slices;
-  if (blocks > INT32_MAX) return MAMBA_E_UNSUPPORTED;
+  if (blocks > 1 << 30) return MAMBA_E_UNSUPPORTED;
+  const dim3 grid((int)std::min<int64_t>(blocks, 1 << kRowBits), (int)((blocks - 1) >> kRowBits) + 1);  // (those behind the last have nothing to do)
   if (l.nseg > 1) {
-    lin_segment_kernel<T, KD, DVT, FIT, EXACT><<<(int)blocks, kThreads, 0, st>>>(l);
+    lin_segment_kernel<T, KD, DVT, FIT, EXACT><<<grid, kThreads, 0, st>>>(l);
     if (hipGetLastError() != hipSuccess) return MAMBA_E_LAUNCH;
   }
-  lin_walk_kernel<T, KD, DVT, FIT, PARTS, EXACT><<<(int)blocks, kThreads, 0, st>>>(l);
+  lin_walk_kernel<T, KD, DVT, FIT, PARTS, EXACT><<<grid, kThreads, 0, st>>>(l);
   return hipGetLastError() == hipSuccess ? MAMBA_OK : MAMBA_E_LAUNCH;
 }
 template <typename T, int KD, int DVT, Fit FIT> int run(const LinLaunch &l, hipStream_t st) {

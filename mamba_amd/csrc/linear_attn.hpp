@@ -41,6 +41,8 @@ struct LinLaunch {
 namespace lin {
 
 constexpr int kThreads = 256, kWaves = 4;
+// A launch takes fewer than 2^32 threads along x: workgroups beyond 2^23 lie along y.
+constexpr int kRowBits = 23;
 
 // The positions that a workgroup walks: [first, first + n) of row `b`, counted in the order of the walk.
 struct Item {
@@ -86,7 +88,7 @@ struct Place {
 DEVI Place place_of(const LinLaunch &p) {
   Place at;
   const int group = p.nheads / p.kv_heads, inner = p.nwalks * p.slices * group;
-  const int xcd = blockIdx.x & 7, r = blockIdx.x >> 3;
+  const int block = blockIdx.y << kRowBits | blockIdx.x, xcd = block & 7, r = block >> 3;
   int in = r % inner;
   const int outer = (r / inner) * 8 + xcd;
   at.none = outer >= p.items * p.kv_heads;

@@ -16,6 +16,7 @@
 namespace {
 
 constexpr int kThreads = 256, kWaves = 4, kHeads = 16;
+constexpr int kRowBits = 23;  // workgroups beyond 2^23 lie along y: a launch takes fewer than 2^32 threads along x
 // workgroups of a CU that the registers leave room for
 constexpr int workgroups(int D) { return D == 64 ? 3 : D == 256 ? 1 : 2; }
 constexpr float kLow = -3e38f;  // stands for a maximum of minus infinity, so that differences are numbers
@@ -68,7 +69,8 @@ template <typename T, int D, bool RAG> __global__ __launch_bounds__(kThreads, RA
   // Workgroups go to the XCDs in turn; all heads of a range (or sequence) are to be on one, as a position's heads lie side by side in
   // memory and share its L2's lines where a head is not whole lines (48 x 12 heads of 80 in fp16: 39 us in order, 37 this way).
   const int rows = p.nkvheads * htiles, n = p.nsplit == 1 ? p.batch : p.nsplit;
-  const int row = n >= 8 ? blockIdx.x / 8 % rows : blockIdx.x % rows, range = n >= 8 ? blockIdx.x / 8 / rows * 8 + blockIdx.x % 8 : blockIdx.x / rows;
+  const uint32_t block = blockIdx.y << kRowBits | blockIdx.x;
+  const int row = n >= 8 ? block / 8 % rows : block % rows, range = n >= 8 ? block / 8 / rows * 8 + block % 8 : block / rows;
   if (range >= n) return;
   const int hk = row / htiles, ht = row % htiles, h0 = hk * group + ht * kHeads, heads = min(group - ht * kHeads, kHeads);
   // tiles [lo, hi) of the batch, of which sequence b begins at `at`
@@ -372,10 +374,11 @@ int size_class(const PagedAttnParams &p) {
 int rows_of_batch(const PagedAttnParams &p) { return p.nkvheads * ((p.nheads / p.nkvheads + kHeads - 1) / kHeads); }
 template <typename T, int D> int run(const PagedAttnParams &p, hipStream_t st) {
   constexpr int V = Frags<T>::V;
-  const int64_t n = p.nsplit == 1 ? p.batch : p.nsplit, grid = rows_of_batch(p) * (n >= 8 ? (n + 7) / 8 * 8 : n);
-  if (grid > INT32_MAX) return MAMBA_E_UNSUPPORTED;
-  if (p.headdim_k % V == 0 && p.headdim_v % V == 0) paged_part_kernel<T, D, false><<<(int)grid, kThreads, 0, st>>>(p);
-  else paged_part_kernel<T, D, true><<<(int)grid, kThreads, 0, st>>>(p);
+  const int64_t n = p.nsplit == 1 ? p.batch : p.nsplit, workgroups = rows_of_batch(p) * (n >= 8 ? (n + 7) / 8 * 8 : n);
+  if (workgroups > 1 << 30 || (p.nsplit > 1 && p.nheads > 1 << kRowBits)) return MAMBA_E_UNSUPPORTED;
+  const dim3 grid((int)std::min<int64_t>(workgroups, 1 << kRowBits), (int)((workgroups - 1) >> kRowBits) + 1);
+  if (p.headdim_k % V == 0 && p.headdim_v % V == 0) paged_part_kernel<T, D, false><<<grid, kThreads, 0, st>>>(p);
+  else paged_part_kernel<T, D, true><<<grid, kThreads, 0, st>>>(p);
   if (hipGetLastError() != hipSuccess) return MAMBA_E_LAUNCH;
   if (p.nsplit > 1) {
     paged_join_kernel<T, D, Frags<T>::KS><<<dim3(p.nheads, p.batch), kThreads, 0, st>>>(p);
