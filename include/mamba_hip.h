@@ -833,7 +833,7 @@ int norm_block_bwd_nparts(const NormBlockParams *p);
  * cu_seqlens (nseq + 1 int32, batch 1, not decreasing) packs nseq sequences into the row: sequence q has the positions
  * cu_seqlens[q] .. cu_seqlens[q + 1] - 1 and starts from its own initial state.  Positions before the first and behind the last
  * sequence count for nothing: their outputs and gradients are 0.
- * Head sizes up to 256, seqlen up to 2^30.  ws: linear_attn_fwd_ws_bytes / linear_attn_bwd_ws_bytes of 16-byte aligned memory
+ * Head sizes up to 256, seqlen up to 2^30, nheads up to 2^22.  ws: linear_attn_fwd_ws_bytes / linear_attn_bwd_ws_bytes of 16-byte aligned memory
  * (0: none), contents ignored on entry, nothing in it is kept between calls.  Every result repeats bit for bit.
  * No result shares memory with an operand, with another result or with ws: workgroups write while others still read.  States that
  * meet (final_states with initial_states, dinitial_states with either) and rows that begin where an operand's do are MAMBA_E_BADARG.

@@ -528,6 +528,7 @@ int check(const LinearAttnParams *p) {
   if (p->nseq < 0 || (p->nseq > 0) != (p->cu_seqlens != nullptr) || (p->nseq > 0 && p->batch != 1)) return MAMBA_E_BADARG;
   if (!(p->scale >= -3.4e38f && p->scale <= 3.4e38f)) return MAMBA_E_BADARG;
   if (p->headdim_k > 256 || p->headdim_v > 256 || p->seqlen > 1 << 30 || p->nseq > 1 << 30) return MAMBA_E_UNSUPPORTED;
+  if (p->nheads > 1 << 22) return MAMBA_E_UNSUPPORTED;  // a position's values are counted in 32 bits
   return MAMBA_OK;
 }
 // Workgroups write results while others still read: states that meet, or rows that begin where an operand's do, are refused.

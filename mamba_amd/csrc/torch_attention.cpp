@@ -121,7 +121,7 @@ pybind11::object linear_attention(const at::Tensor &q, const at::Tensor &k, cons
   const c10::Device dev = q.device();
   if (!heads_ok(q, k, v, dev) || !decay_ok(log_decay, q.size(2), dev)) return no;
   const Linear o{scale_of(scale, q.size(3)), final_states};
-  if (!scale_ok(o.scale) || q.size(0) > INT32_MAX || q.size(1) > (1 << 30)) return no;
+  if (!scale_ok(o.scale) || q.size(0) > INT32_MAX || q.size(1) > (1 << 30) || q.size(2) > (1 << 22)) return no;
   int64_t seqs = q.size(0);
   if (cu) {
     if (!on_device(cu, dev) || cu->scalar_type() != at::kInt || cu->dim() != 1 || cu->size(0) < 2 || cu->size(0) > (1 << 30) ||

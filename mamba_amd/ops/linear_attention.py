@@ -192,8 +192,8 @@ def linear_attention_fn(q, k, v, log_decay, scale=None, initial_states=None, cu_
     what = "linear_attention"
     nheads, nkv, headdim_k, headdim_v = _check_heads(what, q, k, v, ("batch", "seqlen"))
     batch, seqlen = q.shape[:2]
-    if max(batch, nheads) > 2 ** 31 - 1 or seqlen > 2 ** 30:
-        raise RuntimeError(f"{what}: rows of up to 2^30 positions are served, got {seqlen}")
+    if batch > 2 ** 31 - 1 or seqlen > 2 ** 30 or nheads > 2 ** 22:
+        raise RuntimeError(f"{what}: rows of up to 2^30 positions with up to 2^22 heads are served, got {batch} of {seqlen} with {nheads}")
     _check_decay(what, log_decay, nheads)
     scale = _check_scale(what, scale, headdim_k)
     seqs = batch
