@@ -489,7 +489,8 @@ template <typename T, int KD, int DVT, Fit FIT, bool PARTS, bool EXACT> int laun
 template <typename T, int KD, int DVT, Fit FIT> int run(const LinLaunch &l, hipStream_t st) {
   if constexpr (sizeof(T) < 4) {
     const LinWalk &last = l.w[l.nwalks - 1];  // the walk of the values: its state is the result, and heads that share are its sums too
-    if (last.y_f32) return last.end.p ? launch<T, KD, DVT, FIT, true, true>(l, st) : launch<T, KD, DVT, FIT, true, false>(l, st);
+    if constexpr (KD > 64 || DVT == 1)  // (two tiles of 64 keys are a forward pass's: backward both head sizes are keys of a walk)
+      if (last.y_f32) return last.end.p ? launch<T, KD, DVT, FIT, true, true>(l, st) : launch<T, KD, DVT, FIT, true, false>(l, st);
     if (last.end.p) return launch<T, KD, DVT, FIT, false, true>(l, st);
   }
   return launch<T, KD, DVT, FIT, false, false>(l, st);

@@ -11,7 +11,7 @@
 
 namespace {
 
-constexpr int kThreads = 256;
+constexpr int kThreads = 256, LANES = 16;
 
 DEVI float log2_decay(float l) {  // minus infinity is a decay to nothing, above 0 counts as 0, NaN stays
   l = l > 0.f ? 0.f : l;
@@ -54,7 +54,7 @@ template <typename S, int V> struct Piece {
   }
 };
 
-template <typename T, typename S, int LANES> __global__ __launch_bounds__(kThreads) void lin_step_kernel(const LinearAttnStepParams p) {
+template <typename T, typename S> __global__ __launch_bounds__(kThreads) void lin_step_kernel(const LinearAttnStepParams p) {
   constexpr int V = std::is_same_v<S, float> ? 4 : 8, ROWS = kThreads / LANES, U = 8;
   __shared__ float sums[4][LANES * V];
   const int tid = threadIdx.x, lane = tid % LANES, row0 = tid / LANES;
@@ -117,18 +117,17 @@ template <typename T, typename S, int LANES> __global__ __launch_bounds__(kThrea
   }
 }
 
-template <typename T, typename S, int LANES> int run(const LinearAttnStepParams &p, hipStream_t st) {
+template <typename T, typename S> int run(const LinearAttnStepParams &p, hipStream_t st) {
   constexpr int V = std::is_same_v<S, float> ? 4 : 8;
   const dim3 grid((p.headdim_v + LANES * V - 1) / (LANES * V), p.nheads, std::min(p.batch, 65535));
-  lin_step_kernel<T, S, LANES><<<grid, kThreads, 0, st>>>(p);
+  lin_step_kernel<T, S><<<grid, kThreads, 0, st>>>(p);
   return hipGetLastError() == hipSuccess ? MAMBA_OK : MAMBA_E_LAUNCH;
 }
-template <typename T, typename S> int run_lanes(const LinearAttnStepParams &p, hipStream_t st) { return run<T, S, 16>(p, st); }
 template <typename T> int run_state(const LinearAttnStepParams &p, hipStream_t st) {
   switch (p.state_dtype) {
-    case MAMBA_F32: return run_lanes<T, float>(p, st);
-    case MAMBA_BF16: return run_lanes<T, bf16_t>(p, st);
-    default: return run_lanes<T, f16_t>(p, st);
+    case MAMBA_F32: return run<T, float>(p, st);
+    case MAMBA_BF16: return run<T, bf16_t>(p, st);
+    default: return run<T, f16_t>(p, st);
   }
 }
 
