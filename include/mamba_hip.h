@@ -897,7 +897,8 @@ int linear_attn_state_update(const LinearAttnStepParams *p, mamba_stream_t strea
  * nsplit: even ranges of all sequences' positions that are worked on side by side, up to 512 (paged_attn_parts says how many suit; 1:
  * a workgroup per sequence and key head, no workspace);
  * ws: paged_attn_ws_bytes of 16-byte aligned memory, contents ignored on entry.  out shares memory with none of k, v and the caches,
- * and where a token is written no element of one cache is one of the other.  Head sizes up to 256, max_pages * page_size up to 2^30,
+ * and where a token is written no element of one cache is one of the other.  scale is at most 2e38 in size; scores beyond 2.3e38 are
+ * infinities.  Head sizes up to 256, max_pages * page_size up to 2^30,
  * batch up to 65535.
  * ------------------------------------------------------------------------- */
 typedef struct PagedAttnParams {

@@ -19,7 +19,7 @@ constexpr int kThreads = 256, kWaves = 4, kHeads = 16;
 constexpr int kRowBits = 23;  // workgroups beyond 2^23 lie along y: a launch takes fewer than 2^32 threads along x
 // workgroups of a CU that the registers leave room for
 constexpr int workgroups(int D) { return D == 64 ? 3 : D == 256 ? 1 : 2; }
-constexpr float kLow = -3e38f;  // stands for a maximum of minus infinity, so that differences are numbers
+constexpr float kLow = -3.40282347e38f;  // the least number: stands for a maximum of minus infinity, so that differences are numbers
 
 struct Span {  // positions of a sequence, in tiles
   int n;            // positions of the cache before the call; negative: an empty place of the batch
@@ -400,7 +400,7 @@ int check(const PagedAttnParams *p) {
     return MAMBA_E_BADARG;
   if (p->page_size <= 0 || p->num_pages <= 0 || p->max_pages <= 0 || p->window < 0 || p->dtype < MAMBA_F32 || p->dtype > MAMBA_F16)
     return MAMBA_E_BADARG;
-  if (!(p->scale >= -3.4e38f && p->scale <= 3.4e38f)) return MAMBA_E_BADARG;
+  if (!(p->scale >= -2e38f && p->scale <= 2e38f)) return MAMBA_E_BADARG;  // (times log2(e) it is a number too)
   if (p->headdim_k > 256 || p->headdim_v > 256 || (int64_t)p->max_pages * p->page_size > 1 << 30) return MAMBA_E_UNSUPPORTED;
   return MAMBA_OK;
 }

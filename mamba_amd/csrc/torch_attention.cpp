@@ -40,7 +40,7 @@ bool decay_ok(const at::Tensor &l, int64_t heads, const c10::Device &dev) {
   return on_device(l, dev) && l.scalar_type() == at::kFloat && l.dim() == 1 && l.size(0) == heads && l.is_contiguous() && !records(l);
 }
 double scale_of(std::optional<double> scale, int64_t headdim) { return scale ? *scale : 1.0 / std::sqrt((double)headdim); }
-bool scale_ok(double scale) { return std::fabs(scale) <= 3.4e38; }
+bool scale_ok(double scale, double most = 3.4e38) { return std::fabs(scale) <= most; }
 
 // ------------------------------------------------------------------ whole sequences
 struct Linear {
@@ -266,7 +266,7 @@ OptTensor paged_attention(const at::Tensor &q, const OptTensor &k, const OptTens
   if (!counts_ok(lens, dev) || lens.dim() != 1 || lens.size(0) != batch) return std::nullopt;
   if (k_cache.size(1) > (1 << 30) || table.size(1) > (1 << 30) || table.size(1) * k_cache.size(1) > (1 << 30)) return std::nullopt;
   const Paged o{scale_of(scale, dk), window.value_or(0)};
-  if (!scale_ok(o.scale) || (window && (*window < 1 || *window > INT32_MAX))) return std::nullopt;
+  if (!scale_ok(o.scale, 2e38) || (window && (*window < 1 || *window > INT32_MAX))) return std::nullopt;
   if (records(q, k, v, k_cache, v_cache)) return PagedFn::apply(q, k, v, k_cache, v_cache, table, lens, o);
   return paged(q, k, v, k_cache, v_cache, table, lens, o);
 }

@@ -72,10 +72,10 @@ def _check_decay(what, log_decay, nheads):
                            "(mamba_chunk_scan_combined has gradients of its decays)")
 
 
-def _check_scale(what, scale, headdim):
+def _check_scale(what, scale, headdim, most=3.4e38):
     scale = headdim ** -0.5 if scale is None else float(scale)
-    if not abs(scale) <= 3.4e38:
-        raise ValueError(f"{what}: scale must be finite, got {scale}")
+    if not abs(scale) <= most:
+        raise ValueError(f"{what}: scale must be finite, of at most {most:g}, got {scale}")
     return scale
 
 

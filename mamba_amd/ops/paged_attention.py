@@ -83,7 +83,7 @@ def paged_attention_update(q, k, v, k_cache, v_cache, block_table, cache_seqlens
         cache_seqlens: (batch,) int32, positions in the cache before the call: the new token is position cache_seqlens[b].  A negative
             number is a padding entry (nothing written, out = 0); so is an entry without positions.  A number beyond the table's
             positions counts as theirs
-        scale: a number, headdim_k ** -0.5 unless given
+        scale: a number of at most 2e38 in size, headdim_k ** -0.5 unless given.  Scores beyond 2.3e38 are infinities
         window: only the last `window` positions, the new one among them, count; None: all
     Return:
         out: (batch, nheads, headdim_v) in q's dtype
@@ -125,7 +125,7 @@ def paged_attention_update(q, k, v, k_cache, v_cache, block_table, cache_seqlens
         raise RuntimeError(f"{what}: cache_seqlens must be ({batch},) int32")
     if batch > 65535 or num_pages > 2 ** 31 - 1 or block_table.shape[1] * page_size > 2 ** 30:
         raise RuntimeError(f"{what}: up to 65535 sequences and tables of up to 2^30 positions are served")
-    scale = _check_scale(what, scale, headdim_k)
+    scale = _check_scale(what, scale, headdim_k, 2e38)
     if window is not None and not 1 <= int(window) <= 2 ** 31 - 1:
         raise ValueError(f"{what}: window must be at least 1, got {window}")
     _refuse_tangents(what, q, k, v, k_cache, v_cache)

@@ -1,4 +1,5 @@
-"""Linear attention and attention over a paged cache at the ends of their ranges: weights far below the largest one."""
+"""Linear attention and attention over a paged cache at the ends of their ranges: weights far below the largest one,
+scores near the least number."""
 import pytest
 import torch
 
@@ -33,3 +34,18 @@ def test_many_small_weights_beside_a_large_one(batch, low, dtype):
     for row in (0, batch // 2, batch - 1):
         within("out", out[row, 0], ref, bound)
     assert bool((out == out[:1]).all())
+
+
+@pytest.mark.parametrize("positions", [1, 2, 700])
+def test_scores_near_the_least_number(positions):
+    """Scores that are all below -3e38 in units of log2: weights are shares of the largest one as ever."""
+    from mamba_amd.ops.paged_attention import paged_attention_update
+    k = torch.full((positions, 1, 2, 4), 0.0)
+    k[..., 0] = -2.25e19  # times 1e19 times log2(e): -3.25e38
+    v = torch.rand(positions, 1, 2, 4, generator=torch.Generator().manual_seed(0))
+    q = torch.zeros(1, 2, 4)
+    q[..., 0] = 1e19
+    args = [t.cuda() for t in (k, v, torch.arange(positions, dtype=torch.int32)[None], torch.tensor([positions], dtype=torch.int32))]
+    out = paged_attention_update(q.cuda(), None, None, *args, scale=1.0)
+    ref = v.double().mean((0, 1))[None]
+    within("out", out, ref, ref * (32 + 2 * positions) * U)
