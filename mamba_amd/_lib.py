@@ -364,6 +364,14 @@ def current_stream(device):
     return torch.cuda.current_stream(device).cuda_stream
 
 
+def refuse_tangents(what, *tensors):
+    """There are no forward-mode gradients.  torch refuses them only behind a Function's forward, when a state or a cache has been
+    changed already, and what detach() has taken a tangent from it does not refuse at all."""
+    for t in tensors:
+        if t is not None and torch.autograd.forward_ad.unpack_dual(t).tangent is not None:
+            raise NotImplementedError(f"{what} has no forward-mode gradients")
+
+
 def require_gpu(*tensors):
     for t in tensors:
         if t is not None and not t.is_cuda:

@@ -255,6 +255,7 @@ def gated_linear_state_update(state, x, gate_a, gate_x, decay, rate=8.0, state_b
             raise RuntimeError(f"{what}: state_batch_indices must be ({batch},) int32")
     if torch.is_grad_enabled() and state.requires_grad:
         raise RuntimeError(f"{what}: state is updated in place and takes no gradients: detach it, or call under torch.no_grad()")
+    _lib.refuse_tangents(what, state, x, gate_a, gate_x, decay)
     _lib.require_gpu(state, x, gate_a, gate_x, decay, state_batch_indices)
     _one_device(what, x, state, gate_a, gate_x, decay, state_batch_indices)
     if state_batch_indices is not None:

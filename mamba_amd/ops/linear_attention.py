@@ -9,7 +9,6 @@ are held in fp32.  There is no CPU or PyTorch fallback: CPU tensors raise.  `lin
 `linear_attention_state_update_ref` state the arithmetic in plain torch; no operator calls them.
 """
 import torch
-import torch.autograd.forward_ad as fwAD
 
 from mamba_amd import _lib
 
@@ -24,14 +23,6 @@ def _one_device(what, first, *others):
     for t in others:
         if t is not None and t.device != first.device:
             raise RuntimeError(f"{what}: all tensors must be on {first.device}, got one on {t.device}")
-
-
-def _refuse_tangents(what, *tensors):
-    """There are no forward-mode gradients.  torch refuses them only behind a Function's forward, when a state or a cache has been
-    changed already, and what detach() has taken a tangent from it does not refuse at all."""
-    for t in tensors:
-        if t is not None and fwAD.unpack_dual(t).tangent is not None:
-            raise NotImplementedError(f"{what} has no forward-mode gradients")
 
 
 def _int32(t, low, high):
@@ -205,7 +196,7 @@ def linear_attention_fn(q, k, v, log_decay, scale=None, initial_states=None, cu_
         seqs = cu_seqlens.shape[0] - 1
     if initial_states is not None and tuple(initial_states.shape) != (seqs, nheads, headdim_k, headdim_v):
         raise RuntimeError(f"{what}: initial_states must be ({seqs}, {nheads}, {headdim_k}, {headdim_v}), got {tuple(initial_states.shape)}")
-    _refuse_tangents(what, q, k, v, log_decay, initial_states)
+    _lib.refuse_tangents(what, q, k, v, log_decay, initial_states)
     _lib.require_gpu(q, k, v, log_decay, initial_states, cu_seqlens)
     _one_device(what, q, k, v, log_decay, initial_states, cu_seqlens)
     if cu_seqlens is not None:
@@ -290,7 +281,7 @@ def linear_attention_state_update(state, q, k, v, log_decay, scale=None, state_b
             raise RuntimeError(f"{what}: state_batch_indices must be ({batch},) int32")
     if torch.is_grad_enabled() and state.requires_grad:
         raise RuntimeError(f"{what}: state is updated in place and takes no gradients: detach it, or call under torch.no_grad()")
-    _refuse_tangents(what, state, q, k, v, log_decay)
+    _lib.refuse_tangents(what, state, q, k, v, log_decay)
     _lib.require_gpu(state, q, k, v, log_decay, state_batch_indices)
     _one_device(what, q, state, k, v, log_decay, state_batch_indices)
     if state_batch_indices is not None:

@@ -6,7 +6,7 @@ operator calls it.
 import torch
 
 from mamba_amd import _lib
-from mamba_amd.ops.linear_attention import _check_heads, _check_scale, _int32, _one_device, _refuse_tangents, _strides, _unit
+from mamba_amd.ops.linear_attention import _check_heads, _check_scale, _int32, _one_device, _strides, _unit
 
 
 def _rows_apart(t):
@@ -128,7 +128,7 @@ def paged_attention_update(q, k, v, k_cache, v_cache, block_table, cache_seqlens
     scale = _check_scale(what, scale, headdim_k, 2e38)
     if window is not None and not 1 <= int(window) <= 2 ** 31 - 1:
         raise ValueError(f"{what}: window must be at least 1, got {window}")
-    _refuse_tangents(what, q, k, v, k_cache, v_cache)
+    _lib.refuse_tangents(what, q, k, v, k_cache, v_cache)
     _lib.require_gpu(q, k, v, k_cache, v_cache, block_table, cache_seqlens)
     _one_device(what, q, k, v, k_cache, v_cache, block_table, cache_seqlens)
     block_table = _int32(block_table, -1, 2 ** 31 - 1)
