@@ -5,8 +5,12 @@ and the step of one generated token (`linear_attention_state_update`), the count
     S_t = exp(log_decay) * S_{t-1} + k_t v_t^T,    out_t = scale * q_t S_t
 
 per head, with a state of headdim_k x headdim_v.  Keys and values may be shared by neighbouring heads.  The states and every sum
-are held in fp32.  There is no CPU or PyTorch fallback: CPU tensors raise.  `linear_attention_ref` and
-`linear_attention_state_update_ref` state the arithmetic in plain torch; no operator calls them.
+are held in fp32; operands of the matrix products are not, with q in 16 bits.  bf16: a block's scores and the state (initial states
+too) are rounded to bf16, 8 bits, where outputs and gradients are formed from them.  fp16: they keep 16 bits.  Rows that a state takes up keep
+16 bits, and 24 where states are returned (the step: all of them).  fp32: nothing is rounded.
+
+There is no CPU or PyTorch fallback: CPU tensors raise.  `linear_attention_ref` and `linear_attention_state_update_ref` state the
+arithmetic in plain torch; no operator calls them.
 """
 import torch
 
@@ -171,8 +175,9 @@ def linear_attention_fn(q, k, v, log_decay, scale=None, initial_states=None, cu_
         out: (batch, seqlen, nheads, headdim_v) in q's dtype, and with return_final_states also the states after the last
         positions, fp32, of initial_states' shape
 
-    Products are formed in blocks of up to 64 positions of a sequence: an infinity or a NaN at one position makes the outputs of
-    the positions in its block that lie before it NaN too.  Other sequences and heads never see it.
+    Products are formed in blocks of 32 positions (fp32: 16) of a sequence.  An infinity or a NaN in k or v at one position leaves no finite
+    numbers in what it has part in, infinities or NaN: the states and the outputs from there on, and those of the positions in its block that
+    lie before it.  Other sequences and heads never see it.
     """
     ext = _lib.torch_ext()
     if ext is not None:

@@ -1,5 +1,6 @@
 """Attention of one generated token over a paged cache of keys and values, on the HIP kernels (`paged_attention_update`): what
 `selective_state_update` and `causal_conv1d_update` are for the recurrent layers of a hybrid model, for its attention layers.
+Scores and sums are formed in fp32; the weights are rounded to q's type for the product with the values (their sum is not).
 There is no CPU or PyTorch fallback: CPU tensors raise.  `paged_attention_update_ref` states the arithmetic in plain torch; no
 operator calls it.
 """
