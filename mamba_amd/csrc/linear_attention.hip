@@ -12,8 +12,8 @@ using namespace lin;
 // 764 with three; 726 with both in one kernel).
 template <typename F, bool EXACT> using Parts = std::conditional_t<EXACT, typename F::Wider, typename F::Wide>;
 
-// The state of one segment alone, from zero, for the segments behind it: 84 us for 0.22 GB at 8 x 4096 x 20 x 128, a block's latency with
-// 320 workgroups at work.
+// The state of one segment alone, from zero, for the segments behind it: 84-93 us for 0.23 GB at 8 x 4096 x 20 x 128, a block's latency with
+// 320 workgroups at work (of 480: the last segments' states are not asked for).
 template <typename T, int KD, int DVT, Fit FIT, bool EXACT> __global__ __launch_bounds__(kThreads, (Shape<T, KD, DVT>::WORKGROUPS)) void lin_segment_kernel(const LinLaunch p) {
   using F = Frags<T>;
   using Sh = Shape<T, KD, DVT>;
@@ -93,9 +93,11 @@ template <typename T, int KD, int DVT, Fit FIT, bool EXACT> __global__ __launch_
 
 // The walk.  Blocks of 32 positions: their products with one another are 6 of a wave's 56 matrix instructions, the state's own work
 // (scaling it, rounding it to operands) is shared by 32 rows.  Two tiles of values a wave use each operand read from LDS twice.  What
-// bounds it at 8 x 4096 x 20 x 128 in bf16 is memory, then the latency of a block's chain of reads and products: backward 430-455 us
-// for 1.29 GB read and 0.50 written, 364 with every row in L2, 336 without the products; LDS is busy 57 % of it, vector
-// instructions 36 %, matrix instructions 23 %.  Forward 160 (three segments) after 84 for the segments' states.
+// bounds it at 8 x 4096 x 20 x 128 in bf16 is memory, then the latency of a block's chain of reads and products: backward 455-470 us
+// for 1.28 GB read and 0.50 written, 364 with every row in L2, 336 without the products; LDS is busy 57 % of it, vector
+// instructions 36 %, matrix instructions 23 %.  Forward 168 (three segments) after 84-93 for the segments' states.
+// What is rounded for the products: the state and the scores as operands of y to what the results' type shows (F::Comp), as the
+// sums of their products are rounded to that type anyhow; a second part of the state would be 16 more matrix instructions than 56.
 // PARTS: there are walks whose y is a part of a sum, in fp32.  (The loop for those beside the other one costs registers that the
 // launches without them need: 8 spilled a block.)
 template <typename T, int KD, int DVT, Fit FIT, bool PARTS, bool EXACT> __global__ __launch_bounds__(kThreads, (Shape<T, KD, DVT>::WORKGROUPS)) void lin_walk_kernel(const LinLaunch p) {
@@ -389,8 +391,8 @@ __global__ __launch_bounds__(kThreads) void lin_plan_kernel(int4 *plan, const in
 }
 
 // Gradients of heads that share keys and values, added up in order: parts (rows, nheads, dim) in fp32, V columns a thread.  It reads
-// group times 4 bytes for every value it writes: 125 us for dk and dv of 32768 x 32 heads of 64 onto
-// 8, 4.8 TB/s (190 us column by column with divisions of 64 bits).
+// group times 4 bytes for every value it writes: 124-129 us for dk and dv of 32768 x 32 heads of 64 onto
+// 8, 4.7-4.9 TB/s (190 us column by column with divisions of 64 bits).
 template <typename T> DEVI void store4(T *at, f32x4 v) {
   if constexpr (std::is_same_v<T, float>) {
     *(GLOBAL_AS f32x4_a4 *)at = v;
@@ -446,7 +448,8 @@ Cut cut_of(const LinearAttnParams &p, int nwalks) {
   const int64_t seqs = c.packed ? p.nseq : p.batch, chains = (int64_t)p.nheads * nwalks, cus = cu_count();
   const int64_t total = (int64_t)p.batch * p.seqlen, longest = c.packed ? total : p.seqlen;
   // Segments of 128 positions at least: of 64, every segment's own state and the sum of those before it cost as much as the walk
-  // (a row of 777 in bf16, 24 heads: 29 us with 128 and 30 with 64; 2048 in fp32: 38 and 48, 41 with 256).
+  // (a row of 777 in bf16, 24 heads: 29 us with 128 and 30 with 64; 2048 in fp32: 38 and 48, 41 with 256).  Their number is rounded down and their
+  // length up to blocks, so there can be fewer: 777 positions are five of 160.
   constexpr int64_t kLeast = 128;
   // Two tiles of 16 values a wave read a block's rows once for both (8 x 4096 x 20 x 128, backward: 454 us, 510 with one) as long as there are
   // workgroups for the chip with them (that row of 777: 38 us with two, 29 with one).
@@ -459,7 +462,8 @@ Cut cut_of(const LinearAttnParams &p, int nwalks) {
   c.fit = p.headdim_k % v != 0 || p.headdim_v % v != 0 ? ELEMENTS : keys && values ? WHOLE : PIECES;
   // Whole sequences where their walks fill the chip, as the segments' states are one more pass over half of what is read (8 x 4096 x
   // 20 x 128, backward: 454 us in one piece, 585 in two); else as many segments as fill it once (forward, 160 walks for 512 places: 250
-  // us in three pieces, 264 in four, 257 in one).  Packed sequences may be of any length: segments of an even share.
+  // us in three pieces, 264 in four, 257 in one).  Packed sequences may be of any length: segments of an even share.  (What fills the chip is
+  // counted by the keys alone: two tiles of values of 64 keys have two workgroups a CU at a time, not four.)
   const int64_t walks = chains * c.slices, slots = cus * (c.kd == 256 ? 1 : c.kd == 128 ? 2 : 4);
   int64_t len = longest;
   if (seqs * walks < slots) {

@@ -7,7 +7,7 @@
 // As the rows of K sit in memory they are operands; the products leave the tile with 8 positions of one head in a lane, which is
 // the operand that the product with V wants (mma_frag.hpp), and a head's m, l are one lane's; V goes through LDS to be read by
 // columns.  Waves meet at the end, workgroups in a second launch.  Memory bounds it: 131072 positions of 8 x 128 in bf16, 537 MB,
-// 97-103 us (5.2-5.5 TB/s) and 6 for the join; one tile on its way and one at work a wave, two workgroups a CU.
+// 98-105 us (5.1-5.5 TB/s) and 6 for the join; one tile on its way and one at work a wave, two workgroups a CU.
 #include "mma_frag.hpp"
 
 #include <algorithm>
@@ -17,7 +17,9 @@ namespace {
 
 constexpr int kThreads = 256, kWaves = 4, kHeads = 16;
 constexpr int kRowBits = 23;  // workgroups beyond 2^23 lie along y: a launch takes fewer than 2^32 threads along x
-// workgroups of a CU that the registers leave room for
+// workgroups of a CU that the registers leave room for, with rows of whole pieces.  (With others, read element by element, there is room for
+// 2, 1 and 1 at sizes of up to 64, 96 and 128: their ranges take one and a half or two rounds.  32 sequences of up to 8192 positions, 32
+// heads on 8, bf16: 469 us at 100 values a head, 118 at 128.)
 constexpr int workgroups(int D) { return D == 64 ? 3 : D == 256 ? 1 : 2; }
 constexpr float kLow = -3.40282347e38f;  // the least number: stands for a maximum of minus infinity, so that differences are numbers
 
