@@ -93,9 +93,9 @@ template <typename T, int KD, int DVT, Fit FIT, bool EXACT> __global__ __launch_
 
 // The walk.  Blocks of 32 positions: their products with one another are 6 of a wave's 56 matrix instructions, the state's own work
 // (scaling it, rounding it to operands) is shared by 32 rows.  Two tiles of values a wave use each operand read from LDS twice.  What
-// bounds it at 8 x 4096 x 20 x 128 in bf16 is memory, then the latency of a block's chain of reads and products: backward 455-470 us
+// bounds it at 8 x 4096 x 20 x 128 in bf16 is memory, then the latency of a block's chain of reads and products: backward 440-470 us
 // for 1.28 GB read and 0.50 written, 364 with every row in L2, 336 without the products; LDS is busy 57 % of it, vector
-// instructions 36 %, matrix instructions 23 %.  Forward 168 (three segments) after 84-93 for the segments' states.
+// instructions 36 %, matrix instructions 23 %.  Forward 158-168 (three segments) after 84-93 for the segments' states.
 // What is rounded for the products: the state and the scores as operands of y to what the results' type shows (F::Comp), as the
 // sums of their products are rounded to that type anyhow; a second part of the state would be 16 more matrix instructions than 56.
 // PARTS: there are walks whose y is a part of a sum, in fp32.  (The loop for those beside the other one costs registers that the
