@@ -98,6 +98,9 @@ template <typename T, int KD, int DVT, Fit FIT, bool EXACT> __global__ __launch_
 // instructions 36 %, matrix instructions 23 %.  Forward 158-168 (three segments) after 84-93 for the segments' states.
 // What is rounded for the products: the state and the scores as operands of y to what the results' type shows (F::Comp), as the
 // sums of their products are rounded to that type anyhow; a second part of the state would be 16 more matrix instructions than 56.
+// A score's rounding is all of its row's values': in a sequence of a few positions nothing evens it out, and 1.5 times the error of one
+// rounding of the results was seen.  So the blocks at a sequence's end (all of a short one) take the scores in two parts.  (In every
+// block: 450-457 / 166 us in place of 428 / 159; with the parts side by side, 102 in place of 97 for the packed forward pass.)
 // PARTS: there are walks whose y is a part of a sum, in fp32.  (The loop for those beside the other one costs registers that the
 // launches without them need: 8 spilled a block.)
 template <typename T, int KD, int DVT, Fit FIT, bool PARTS, bool EXACT> __global__ __launch_bounds__(kThreads, (Shape<T, KD, DVT>::WORKGROUPS)) void lin_walk_kernel(const LinLaunch p) {
@@ -224,7 +227,7 @@ template <typename T, int KD, int DVT, Fit FIT, bool PARTS, bool EXACT> __global
     for (int kb = 0; kb < KB; ++kb) acc = F::mma_raw(lanes.along_krow(br, kb), lanes.along(ar, kb), acc);
 #pragma unroll
     for (int r = 0; r < 4; ++r) acc[r] = r <= first ? acc[r] * pair[r] : 0.f;
-    F::store_comp(reinterpret_cast<typename F::Comp *>(to) + tile * 64 + lane, half, acc);
+    F::template store_wide<Sh::BLOCKS * 64>(to, tile * 64 + lane, half, acc);
   };
 
   // whole blocks of near rows: the lowest row of a turn, from turn to turn, the thread's place (bytes)
@@ -276,9 +279,12 @@ template <typename T, int KD, int DVT, Fit FIT, bool PARTS, bool EXACT> __global
 #pragma unroll
       for (int ib = 0; ib < IT; ++ib) {
         if (jb * KS > ib * 16 + 15) continue;
-        const typename F::Comp s = reinterpret_cast<const typename F::Comp *>(s_now)[Sh::block_of(ib, jb) * 64 + lane];
+        auto with = [&](const auto &s) {
 #pragma unroll
-        for (int d = 0; d < DVT; ++d) y[ib][d] = mma16(cd[d], s, y[ib][d]);
+          for (int d = 0; d < DVT; ++d) y[ib][d] = mma16(cd[d], s, y[ib][d]);
+        };
+        if constexpr (FULL) with(F::template load_comp<Sh::BLOCKS * 64>(s_now, Sh::block_of(ib, jb) * 64 + lane));
+        else with(F::template load_wide<Sh::BLOCKS * 64>(s_now, Sh::block_of(ib, jb) * 64 + lane));
       }
     }
 #pragma unroll

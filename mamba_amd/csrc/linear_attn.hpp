@@ -208,7 +208,7 @@ template <typename T, int KD, int DVT> struct Shape {
   static_assert(BLOCKS * F::NT <= kWaves, "a tile of scores a wave");
   // LDS, bytes: rows a, b, c of a stage, two of them; decayed scores, twice; y
   static constexpr int B = F::size(C, KD), CC = 2 * B, STAGE = CC + F::size(C, VAL);
-  static constexpr int SCORES = BLOCKS * 64 * (int)sizeof(typename F::Comp), AT_SCORES = 2 * STAGE, AT_Y = AT_SCORES + 2 * SCORES;
+  static constexpr int SCORES = BLOCKS * 64 * (int)sizeof(typename F::Wide), AT_SCORES = 2 * STAGE, AT_Y = AT_SCORES + 2 * SCORES;
   static constexpr int LDS = AT_Y + F::size(C, VAL);
   // workgroups of a CU: what the LDS has room for and what the registers hold without spills (128, 256 or 512 a lane)
   static constexpr int ROOM = 160 * 1024 / LDS, MOST = TILES <= 4 ? 4 : KD <= 128 ? 2 : 1;

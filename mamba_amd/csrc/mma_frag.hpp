@@ -119,6 +119,17 @@ template <typename T> struct Frags16 {
     const frag_i16x4 lo = lds_transposed(reinterpret_cast<const uint16_t *>(rows)), hi = lds_transposed(reinterpret_cast<const uint16_t *>(rows4));
     return __builtin_bit_cast(u32x4, (frag_i16x8)__builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
   }
+  // Computed fragments of N lanes in LDS, the first parts of all of them before the second ones: what a lane holds of a tile of results
+  // becomes the tile `half` of fragment n.
+  template <int N> static DEVI void store_wide(char *at, int n, int half, f32x4 v) {
+    const u32x2 hi = {pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3])};
+    reinterpret_cast<u32x2 *>(at + 16 * n)[half] = hi;
+    reinterpret_cast<u32x2 *>(at + 16 * (N + n))[half] = u32x2{pack_bf16(v[0] - bf16_lo(hi[0]), v[1] - bf16_hi(hi[0])), pack_bf16(v[2] - bf16_lo(hi[1]), v[3] - bf16_hi(hi[1]))};
+  }
+  template <int N> static DEVI Split load_wide(const char *at, int n) {
+    const frag_bf16x8 *of = reinterpret_cast<const frag_bf16x8 *>(at);
+    return Split{of[n], of[N + n]};
+  }
   static DEVI void gather(const f32x4 (&t)[2], float (&v)[8]) {
 #pragma unroll
     for (int e = 0; e < 4; ++e) v[e] = t[0][e], v[4 + e] = t[1][e];
@@ -138,18 +149,15 @@ template <> struct Frags<bf16_t> : Frags16<bf16_t> {
 #pragma unroll
     for (int e = 0; e < 4; ++e) v[2 * e] = bf16_lo(w[e]), v[2 * e + 1] = bf16_hi(w[e]);
   }
-  // What a lane holds of a tile of results: into row `row` of a tile in LDS, as the columns 16 n + 4 g .. ..
+  // what a lane holds of a tile of results, into row `row` of a tile in LDS as the columns 16 n + 4 g ..
   template <int COLS> static DEVI void store(char *tile, int row, int n, int g, f32x4 v) {
     *reinterpret_cast<u32x2 *>(tile + 2 * (place<COLS>(row, 2 * n + (g >> 1)) + 4 * (g & 1))) = u32x2{pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3])};
-  }
-  // .. or as the tile `half` of the lane's computed fragment
-  static DEVI void store_comp(Comp *frag, int half, f32x4 v) {
-    reinterpret_cast<u32x2 *>(frag)[half] = u32x2{pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3])};
   }
   static DEVI u32x4 pack(const float (&v)[8]) {
     return u32x4{pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3]), pack_bf16(v[4], v[5]), pack_bf16(v[6], v[7])};
   }
   static DEVI Comp comp(const float (&v)[8]) { return data(pack(v)); }
+  template <int N> static DEVI Comp load_comp(const char *at, int n) { return reinterpret_cast<const frag_bf16x8 *>(at)[n]; }
   template <typename W> static DEVI W wide(const float (&v)[8]) {
     W s;
     s.set(v);
@@ -168,11 +176,6 @@ template <> struct Frags<f16_t> : Frags16<f16_t> {
   }
   template <int COLS> static DEVI void store(char *tile, int row, int n, int g, f32x4 v) {
     *reinterpret_cast<u32x2 *>(tile + 2 * (place<COLS>(row, 2 * n + (g >> 1)) + 4 * (g & 1))) = u32x2{pack_f16(v[0], v[1]), pack_f16(v[2], v[3])};
-  }
-  static DEVI void store_comp(Comp *frag, int half, f32x4 v) {
-    const u32x2 hi = {pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3])};
-    reinterpret_cast<u32x2 *>(&frag->h)[half] = hi;
-    reinterpret_cast<u32x2 *>(&frag->l)[half] = u32x2{pack_bf16(v[0] - bf16_lo(hi[0]), v[1] - bf16_hi(hi[0])), pack_bf16(v[2] - bf16_lo(hi[1]), v[3] - bf16_hi(hi[1]))};
   }
   static DEVI u32x4 pack(const float (&v)[8]) {
     return u32x4{pack_f16(v[0], v[1]), pack_f16(v[2], v[3]), pack_f16(v[4], v[5]), pack_f16(v[6], v[7])};
@@ -195,6 +198,7 @@ template <> struct Frags<f16_t> : Frags16<f16_t> {
     s.set(v);
     return s;
   }
+  template <int N> static DEVI Comp load_comp(const char *at, int n) { return load_wide<N>(at, n); }
 };
 template <> struct Frags<float> {
   using E = float;
@@ -237,7 +241,9 @@ template <> struct Frags<float> {
     for (int e = 0; e < 4; ++e) v[e] = w[e];
   }
   template <int COLS> static DEVI void store(char *tile, int row, int n, int g, f32x4 v) { *reinterpret_cast<f32x4 *>(tile + 4 * place<COLS>(row, 4 * n + g)) = v; }
-  static DEVI void store_comp(Comp *frag, int, f32x4 v) { frag->v = v; }
+  template <int N> static DEVI void store_wide(char *at, int n, int, f32x4 v) { reinterpret_cast<f32x4 *>(at)[n] = v; }
+  template <int N> static DEVI Frag32 load_wide(const char *at, int n) { return Frag32{reinterpret_cast<const f32x4 *>(at)[n]}; }
+  template <int N> static DEVI Frag32 load_comp(const char *at, int n) { return load_wide<N>(at, n); }
   static DEVI f32x4 pack(const float (&v)[4]) { return f32x4{v[0], v[1], v[2], v[3]}; }
   static DEVI Frag32 comp(const float (&v)[4]) { return Frag32{f32x4{v[0], v[1], v[2], v[3]}}; }
   template <typename W> static DEVI W wide(const float (&v)[4]) { return comp(v); }

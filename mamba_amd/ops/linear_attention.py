@@ -6,7 +6,8 @@ and the step of one generated token (`linear_attention_state_update`), the count
 
 per head, with a state of headdim_k x headdim_v.  Keys and values may be shared by neighbouring heads.  The states and every sum
 are held in fp32; operands of the matrix products are not, with q in 16 bits.  bf16: a block's scores and the state (initial states
-too) are rounded to bf16, 8 bits, where outputs and gradients are formed from them.  fp16: they keep 16 bits.  Rows that a state takes up keep
+too) are rounded to bf16, 8 bits, where outputs and gradients are formed from them (the scores of a sequence's last blocks, or of a
+sequence of fewer than 96 positions, keep 16).  fp16: they keep 16 bits.  Rows that a state takes up keep
 16 bits, and 24 where states are returned (the step: all of them).  fp32: nothing is rounded.
 
 There is no CPU or PyTorch fallback: CPU tensors raise.  `linear_attention_ref` and `linear_attention_state_update_ref` state the

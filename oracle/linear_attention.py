@@ -13,10 +13,11 @@ the same sum of absolute values, and the result is off by a number of steps time
    from the blocks before, 2 * 378; its exponential, products and scale, 16; and once per block (of 32 positions or more) that a
    state has gone through, its factor and the product with it, 6 u + 3 u |x|, where the x of all blocks together count once more
    as above, 378.  K = 1800 + 6 (n / 32 + 1) for a sequence of n positions.
- * What is rounded on its way from one product to the next.  bf16: the decayed scores and the state, as operands of out, dq, dk
-   and dv, to 8 bits, 2^-8 of each; the decayed values that a state takes up, in two parts, 2^-16.  fp16: everything computed, in two
-   parts, with the products of two second parts left out, 2^-15.  Where a state is a result, the values it takes up are in three parts,
-   and in fp16 the products of second and third parts are left out, 2^-23.  fp32: nothing.  Gradients of shared heads are sums in fp32.
+ * What is rounded on its way from one product to the next.  bf16: the decayed scores (at a sequence's end in two parts) and the
+   state, as operands of out, dq, dk and dv, to 8 bits, 2^-8 of each; the decayed values that a state takes up, in two parts, 2^-16.
+   fp16: everything computed, in two parts, with the products of two second parts left out, 2^-15.  Where a state is a result, the
+   values it takes up are in three parts, and in fp16 the products of second and third parts are left out, 2^-23.  fp32: nothing.
+   Gradients of shared heads are sums in fp32.
    (K covers sums of any numbers; tests/test_linear_attention_precision_gpu.py has results of one product each, to a fortieth of it.)
 
 Attention.  A score is off by d = (headdim_k + 8) u scale |q| . |k|, its weight 2^(..) relative to the others by 2 d and 16 u; the

@@ -72,6 +72,26 @@ def test_states_that_are_results_in_16_bit_types(L, size, first, dtype):
     within("dinitial", mirrored["dinitial"], ref["dinitial"], _bound(ref["dinitial"], L - first, 2, 1, 1))
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("batch,L,heads,kv,dk,dv", [(1, 1, 1, 1, 1, 1), (5, 1, 32, 4, 96, 48), (1, 2, 4, 4, 16, 16), (2, 31, 4, 2, 64, 64), (1, 32, 2, 2, 128, 128),
+                                                   (1, 32, 2, 2, 256, 40), (3, 17, 3, 3, 33, 7)])
+def test_results_of_one_block_are_rounded_once(batch, L, heads, kv, dk, dv, dtype):
+    """Without a state that comes in, a block's results are products of its scores, which are held in two bf16 parts (2^-16 of them; in
+    fp16 the products of two second parts are left out, 2^-16 more): what is seen is the rounding of the result."""
+    from mamba_amd.ops.linear_attention import linear_attention_fn
+    g = torch.Generator().manual_seed(L + dk)
+    r = lambda h, d: torch.randn(batch, L, h, d, generator=g).to(dtype)
+    q, k, v, dout, decay = r(heads, dk), r(kv, dk), r(kv, dv), r(heads, dv), torch.log1p(-torch.exp2(-torch.linspace(1, 12, heads)))
+    ref, _ = linear_attention_oracle(q, k, v, decay, dout=dout)
+    # sums of absolute values: the same of absolute operands
+    size, _ = linear_attention_oracle(q.abs(), k.abs(), v.abs(), decay, dout=dout.abs())
+    leaves = [t.cuda().requires_grad_() for t in (q, k, v)]
+    out = linear_attention_fn(*leaves, decay.cuda())
+    for n, x in zip(("out", "dq", "dk", "dv"), (out, *torch.autograd.grad(out, leaves, dout.cuda()))):
+        within(n, x, ref[n], size[n] * (2.0 ** -15 + (dk + dv + 32 + 60) * U))
+
+
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
 @pytest.mark.parametrize("L", [24, 32])
 def test_the_bound_tells_two_parts_from_three(dtype, L):
