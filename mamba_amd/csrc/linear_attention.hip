@@ -12,7 +12,7 @@ using namespace lin;
 // 764 with three; 726 with both in one kernel).
 template <typename F, bool EXACT> using Parts = std::conditional_t<EXACT, typename F::Wider, typename F::Wide>;
 
-// The state of one segment alone, from zero, for the segments behind it: 84-93 us for 0.23 GB at 8 x 4096 x 20 x 128, a block's latency with
+// The state of one segment alone, from zero, for the segments behind it: 81-93 us for 0.23 GB at 8 x 4096 x 20 x 128, a block's latency with
 // 320 workgroups at work (of 480: the last segments' states are not asked for).
 template <typename T, int KD, int DVT, Fit FIT, bool EXACT> __global__ __launch_bounds__(kThreads, (Shape<T, KD, DVT>::WORKGROUPS)) void lin_segment_kernel(const LinLaunch p) {
   using F = Frags<T>;
@@ -93,9 +93,9 @@ template <typename T, int KD, int DVT, Fit FIT, bool EXACT> __global__ __launch_
 
 // The walk.  Blocks of 32 positions: their products with one another are 6 of a wave's 56 matrix instructions, the state's own work
 // (scaling it, rounding it to operands) is shared by 32 rows.  Two tiles of values a wave use each operand read from LDS twice.  What
-// bounds it at 8 x 4096 x 20 x 128 in bf16 is memory, then the latency of a block's chain of reads and products: backward 440-470 us
+// bounds it at 8 x 4096 x 20 x 128 in bf16 is memory, then the latency of a block's chain of reads and products: backward 430-475 us
 // for 1.28 GB read and 0.50 written, 364 with every row in L2, 336 without the products; LDS is busy 57 % of it, vector
-// instructions 36 %, matrix instructions 23 %.  Forward 158-168 (three segments) after 84-93 for the segments' states.
+// instructions 36 %, matrix instructions 23 %.  Forward 155-170 (three segments) after 81-93 for the segments' states.
 // What is rounded for the products: the state and the scores as operands of y to what the results' type shows (F::Comp), as the
 // sums of their products are rounded to that type anyhow; a second part of the state would be 16 more matrix instructions than 56.
 // A score's rounding is all of its row's values': in a sequence of a few positions nothing evens it out, and 1.5 times the error of one
